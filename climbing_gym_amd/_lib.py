@@ -63,6 +63,10 @@ _SIGNATURES = {
     "lfm2_record_sample": "ppppppppppppppp" "llllp",
     "lfm2_sample_record": "pppppppppppppppppppp" "llllip",
     "lfm2_record_head": "pppppp" "illp",
+    "lfm2_token_logprobs": "pppp" "l" "pp" "fllip",
+    "lfm2_token_logprobs_backward": "pl" "pl" "ppppp" "fllip",
+    "lfm2_policy_loss": "pppppppppppp" "lliii" "fffff" "p",
+    "lfm2_policy_gradient": "ppppp" "l" "p" "l" "ppppppp" "f" "p" "llliii" "ffffff" "ip",
     "lfm2_hbm_stream_read": "plpiip",
     "lfm2_mfma_fp8_peak": "ppiiip",
     "lfm2_timestamp": "pp",
@@ -76,6 +80,7 @@ _INT64_RESULT = {
     "lfm2_bf16_gemm_workspace": "lll",
     "lfm2_decode_attention_workspace": "liil",
     "lfm2_decode_schedule_size": "ll",
+    "lfm2_policy_workspace": "lli",
     "lfm2_timestamp_rate_khz": "",
 }
 _CTYPE = {"p": ctypes.c_void_p, "l": ctypes.c_int64, "i": ctypes.c_int, "f": ctypes.c_float}

@@ -691,6 +691,271 @@ def record_head(ids, probs, out_ids, out_probs, lengths, alive, k: int, cap: int
          int(cap), lengths.numel())
 
 
+# ----------------------------------------------------------------------------------- scoring and policy loss
+def _one_device(*tensors):
+    """The device all given tensors (None: left out) live on; the launch goes to that device's current stream."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        reject(not t.is_cuda, "HIP kernels require GPU tensors")
+        reject(device is not None and t.device != device, "all tensors of a call live on one device")
+        device = t.device
+    return device
+
+
+def _call_on(device, name: str, *args) -> None:
+    if device.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
+
+
+def _check_logits(logits, targets, temperature):
+    reject(logits.ndim != 2 or not logits.is_cuda or logits.dtype not in DTYPE_CODE,
+           "scoring requires a 2D GPU BF16/FP16/FP32 logits tensor")
+    reject(logits.size(1) == 0 or (logits.size(1) > 1 and logits.stride(1) != 1) or (logits.size(0) > 1 and logits.stride(0) < logits.size(1)),
+           "logits need at least one column, consecutive columns and rows that do not overlap")
+    _check_row_values(targets, logits.size(0), torch.long, "targets")
+    if isinstance(temperature, torch.Tensor):
+        _check_row_values(temperature, logits.size(0), torch.float32, "temperature")
+        return temperature, 1.0
+    reject(not 0.0 < float(temperature) < float("inf"), "temperature must be positive and finite, or an fp32 tensor with one entry per row")
+    return None, float(temperature)
+
+
+def _check_row_values(tensor, rows: int, dtype, name: str) -> None:
+    reject(not isinstance(tensor, torch.Tensor) or tensor.dtype != dtype or tensor.shape != (rows,) or not tensor.is_contiguous(),
+           f"{name} must be a contiguous {dtype} tensor of {rows} entries")
+
+
+def _row_stride(matrix) -> int:
+    return matrix.stride(0) if matrix.size(0) > 1 else matrix.size(1)
+
+
+def _gradient_output(out, logits):
+    """The tensor a gradient of the logits goes to: fresh, or `out` (the logits themselves, or memory apart from them)."""
+    if out is None:
+        return torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+    reject(out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device
+           or (out.size(1) > 1 and out.stride(1) != 1) or (out.size(0) > 1 and out.stride(0) < out.size(1)),
+           "out must match the logits in shape, dtype and device, with consecutive columns and rows that do not overlap")
+    same = out.data_ptr() == logits.data_ptr() and _row_stride(out) == _row_stride(logits)
+    reject(not same and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr(),
+           "out must be the logits themselves or share no storage with them")
+    return out
+
+
+def token_logprobs_forward(logits: torch.Tensor, targets: torch.Tensor, *, temperature=1.0, entropy: bool = False):
+    """log softmax(logits / temperature) at `targets` in one pass over the logits, where lfm25_engine.py:1108-1163 makes an
+    fp32 copy and runs logsumexp and gather: returns (log-probabilities fp32 [N], entropies fp32 [N] or None, row
+    statistics fp32 [N, 4] for `token_logprobs_backward`).  `logits` [N, V] may be rows of a wider matrix; `targets` int64,
+    a negative one takes its row out (zeros), one outside the vocabulary gives NaN; `temperature` a number or fp32 [N]
+    (rows with a temperature <= 0 are scored at 1).  Rows of -inf only give -inf and entropy 0."""
+    temperatures, value = _check_logits(logits, targets, temperature)
+    device, rows = _one_device(logits, targets, temperatures), logits.size(0)
+    logprobs = torch.empty(rows, device=device, dtype=torch.float32)
+    entropies = torch.empty(rows, device=device, dtype=torch.float32) if entropy else None
+    stats = torch.empty((rows, 4), device=device, dtype=torch.float32)
+    if rows:
+        _call_on(device, "lfm2_token_logprobs", logprobs, entropies, stats, logits, _row_stride(logits), targets, temperatures,
+                 value, rows, logits.size(1), _code(logits.dtype))
+    return logprobs, entropies, stats
+
+
+def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, stats: torch.Tensor, grad_logprobs: torch.Tensor,
+                            grad_entropy: torch.Tensor | None = None, *, temperature=1.0, out: torch.Tensor | None = None):
+    """Gradient of the logits for `grad_logprobs` and, after a forward call with `entropy=True`, `grad_entropy` (fp32 [N]),
+    with the logits, targets and temperature of that call; rounded once to the logits' dtype.  `out` may be the logits."""
+    temperatures, value = _check_logits(logits, targets, temperature)
+    rows = logits.size(0)
+    reject(stats.dtype != torch.float32 or stats.shape != (rows, 4) or not stats.is_contiguous(),
+           "stats must be the fp32 [rows, 4] statistics of token_logprobs_forward")
+    _check_row_values(grad_logprobs, rows, torch.float32, "grad_logprobs")
+    if grad_entropy is not None:
+        _check_row_values(grad_entropy, rows, torch.float32, "grad_entropy")
+    device = _one_device(logits, targets, temperatures, stats, grad_logprobs, grad_entropy)
+    grad = _gradient_output(out, logits)
+    if rows:
+        _call_on(device, "lfm2_token_logprobs_backward", grad, _row_stride(grad), logits, _row_stride(logits), targets, stats,
+                 grad_logprobs, grad_entropy, temperatures, value, rows, logits.size(1), _code(logits.dtype))
+    return grad
+
+
+def _refuse_captured_graph(*tensors) -> None:
+    """An autograd graph recorded while a HIP graph is captured ties the capture to leaves that eager graphs also hold, and
+    its backward then runs on their streams; the explicit forward and backward calls have no such graph."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        reject(torch.cuda.is_current_stream_capturing(),
+               "inside a graph capture, call the explicit forward and backward functions instead of autograd", RuntimeError)
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, temperature, entropy):
+        logprobs, entropies, stats = token_logprobs_forward(logits, targets, temperature=temperature, entropy=entropy)
+        per_row = isinstance(temperature, torch.Tensor)
+        ctx.save_for_backward(logits, targets, stats, temperature if per_row else None)
+        ctx.temperature = None if per_row else temperature
+        ctx.set_materialize_grads(False)
+        return (logprobs, entropies) if entropy else logprobs
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_logprobs, grad_entropy=None):
+        reject(torch.cuda.is_current_stream_capturing(),
+               "inside a graph capture, call token_logprobs_backward instead of autograd", RuntimeError)
+        logits, targets, stats, temperatures = ctx.saved_tensors
+        if grad_logprobs is None and grad_entropy is None:
+            return None, None, None, None
+        if grad_logprobs is None:
+            grad_logprobs = torch.zeros_like(grad_entropy)
+        grad = token_logprobs_backward(logits, targets, stats, grad_logprobs.contiguous(),
+                                       None if grad_entropy is None else grad_entropy.contiguous(),
+                                       temperature=temperatures if ctx.temperature is None else ctx.temperature)
+        return grad, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, temperature=1.0, entropy: bool = False):
+    """`token_logprobs_forward` for autograd: log-probabilities, or (log-probabilities, entropies), differentiable in the
+    logits (once; the temperature is a constant).  Inside a graph capture use the explicit pair."""
+    _refuse_captured_graph(logits)
+    return _TokenLogprobs.apply(logits, targets, temperature, bool(entropy))
+
+
+_AGGREGATE = {"token": 0, "sequence": 1, "sum": 2}
+_KL = {"k1": 1, "k2": 2, "k3": 3}
+
+
+@dataclass(frozen=True)
+class PolicyLossConfig:
+    """Clipped policy loss: the ratio is cut to [1 - clip_low, 1 + clip_high]; with `dual_clip` (> 1) the gain of a token
+    with a negative advantage is bounded below by dual_clip * advantage; `kl_coef` weighs the KL estimate to the reference
+    policy (k1: logp - ref, k2: half its square, k3: e^x - 1 - x with x = ref - logp), `entropy_coef` an entropy bonus.
+    `aggregate`: mean over all tokens that count ("token"), mean over sequences of their token means ("sequence"), "sum"."""
+    clip_low: float = 0.2
+    clip_high: float = 0.2
+    dual_clip: Optional[float] = None
+    kl: str = "k3"
+    kl_coef: float = 0.0
+    entropy_coef: float = 0.0
+    aggregate: str = "token"
+
+    def __post_init__(self):
+        finite = lambda v: -float("inf") < float(v) < float("inf")
+        reject(not 0.0 <= self.clip_low < 1.0, "clip_low must be in [0, 1)")
+        reject(not (finite(self.clip_high) and self.clip_high >= 0.0), "clip_high must be finite and >= 0")
+        reject(self.dual_clip is not None and not (finite(self.dual_clip) and self.dual_clip > 1.0), "dual_clip must be above 1")
+        reject(self.kl not in _KL, f"kl must be one of {sorted(_KL)}")
+        reject(self.aggregate not in _AGGREGATE, f"aggregate must be one of {sorted(_AGGREGATE)}")
+        reject(not finite(self.kl_coef) or not finite(self.entropy_coef), "coefficients must be finite")
+
+    def _arguments(self):
+        return (_AGGREGATE[self.aggregate], _KL[self.kl], float(self.clip_low), float(self.clip_high), float(self.dual_clip or 0.0),
+                float(self.kl_coef), float(self.entropy_coef))
+
+
+def _check_tokens(tokens: int, old_logprobs, advantages, mask, ref_logprobs, cu_seqlens, per_sequence: bool, config):
+    """Arguments the two forms of the loss share; returns the sequence count."""
+    _check_row_values(old_logprobs, tokens, torch.float32, "old_logprobs")
+    if ref_logprobs is not None:
+        _check_row_values(ref_logprobs, tokens, torch.float32, "ref_logprobs")
+    reject(config.kl_coef != 0.0 and ref_logprobs is None, "a KL term needs ref_logprobs")
+    if mask is not None:
+        reject(mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (tokens,) or not mask.is_contiguous(),
+               f"mask must be a contiguous bool tensor of {tokens} entries")
+    sequences = 1
+    if cu_seqlens is not None:
+        reject(cu_seqlens.dtype != torch.int32 or cu_seqlens.ndim != 1 or cu_seqlens.numel() < 2 or not cu_seqlens.is_contiguous(),
+               "cu_seqlens must be a contiguous int32 tensor of at least two bounds")
+        sequences = cu_seqlens.numel() - 1
+    _check_row_values(advantages, sequences if per_sequence else tokens, torch.float32, "advantages")
+    return sequences
+
+
+def policy_loss_forward(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, *,
+                        mask: torch.Tensor | None = None, ref_logprobs: torch.Tensor | None = None,
+                        entropy: torch.Tensor | None = None, cu_seqlens: torch.Tensor | None = None, per_sequence: bool = False,
+                        config: PolicyLossConfig = PolicyLossConfig()):
+    """Clipped policy loss over packed completions (see `PolicyLossConfig`) and its gradient: returns (loss fp32 scalar,
+    stats fp32 [7], d loss / d logprobs fp32 [N], d loss / d entropy fp32 [N] or None).  Everything per token is fp32 [N];
+    `mask` (bool) says which tokens count; sequence i is tokens cu_seqlens[i] .. cu_seqlens[i+1] - 1 (int32; None: one
+    sequence), tokens behind the last one do not count; `advantages` has one entry per token, or per sequence with
+    `per_sequence`.  What tokens that do not count hold (NaN included) is not used and their gradient is 0.
+    stats = weighted policy term, weighted KL, weighted entropy, share of ratios cut, mean ratio, mean of r - 1 - log r,
+    number of tokens that count."""
+    tokens = logprobs.numel()
+    _check_row_values(logprobs, tokens, torch.float32, "logprobs")
+    sequences = _check_tokens(tokens, old_logprobs, advantages, mask, ref_logprobs, cu_seqlens, per_sequence, config)
+    if entropy is not None:
+        _check_row_values(entropy, tokens, torch.float32, "entropy")
+    reject(config.entropy_coef != 0.0 and entropy is None, "an entropy bonus needs the tokens' entropies")
+    device = _one_device(logprobs, old_logprobs, advantages, mask, ref_logprobs, entropy, cu_seqlens)
+    fresh = lambda *shape: torch.empty(shape, device=device, dtype=torch.float32)
+    if tokens == 0:
+        return (torch.zeros((), device=device), torch.zeros(7, device=device), fresh(0), None if entropy is None else fresh(0))
+    loss, stats, grad = fresh(), fresh(7), fresh(tokens)
+    grad_entropy = None if entropy is None else fresh(tokens)
+    workspace = fresh(query("lfm2_policy_workspace", tokens, sequences, int(cu_seqlens is not None)))
+    _call_on(device, "lfm2_policy_loss", loss, stats, grad, grad_entropy, logprobs, old_logprobs, advantages, ref_logprobs, entropy,
+             mask, cu_seqlens, workspace, tokens, sequences, int(per_sequence), *config._arguments())
+    return loss, stats, grad, grad_entropy
+
+
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logprobs, entropy, old_logprobs, advantages, mask, ref_logprobs, cu_seqlens, per_sequence, config):
+        loss, stats, grad, grad_entropy = policy_loss_forward(
+            logprobs, old_logprobs, advantages, mask=mask, ref_logprobs=ref_logprobs, entropy=entropy, cu_seqlens=cu_seqlens,
+            per_sequence=per_sequence, config=config)
+        ctx.save_for_backward(grad, grad_entropy)
+        ctx.mark_non_differentiable(stats)
+        return loss, stats
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss, _):
+        reject(torch.cuda.is_current_stream_capturing(),
+               "inside a graph capture, use the gradient that policy_loss_forward returns instead of autograd", RuntimeError)
+        grad, grad_entropy = ctx.saved_tensors
+        return (grad * grad_loss, None if grad_entropy is None else grad_entropy * grad_loss, *[None] * 7)
+
+
+def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, *, mask=None, ref_logprobs=None,
+                entropy=None, cu_seqlens=None, per_sequence: bool = False, config: PolicyLossConfig = PolicyLossConfig()):
+    """`policy_loss_forward` for autograd: (loss, stats), the loss differentiable (once) in `logprobs` and `entropy`; the
+    other arguments are constants and `stats` carries no gradient."""
+    _refuse_captured_graph(logprobs, entropy)
+    return _PolicyLoss.apply(logprobs, entropy, old_logprobs, advantages, mask, ref_logprobs, cu_seqlens, bool(per_sequence), config)
+
+
+def policy_gradient(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, *,
+                    mask=None, ref_logprobs=None, cu_seqlens=None, per_sequence: bool = False, temperature=1.0,
+                    config: PolicyLossConfig = PolicyLossConfig(), grad_scale: float = 1.0, out: torch.Tensor | None = None):
+    """`token_logprobs`, `policy_loss` and the gradient of the logits in one pass over the rows that count, without the
+    second reading of the logits that a backward call makes: returns (loss, stats, log-probabilities fp32 [N],
+    grad_scale * d loss / d logits in the logits' dtype).  Arguments as in those two functions; a token counts when `mask`
+    says so and its target is not negative; rows that do not count get zeros.  For `logits.backward(gradient)` of the
+    caller's own graph.  `out` (where the gradient goes) may be the logits."""
+    temperatures, value = _check_logits(logits, targets, temperature)
+    tokens = logits.size(0)
+    sequences = _check_tokens(tokens, old_logprobs, advantages, mask, ref_logprobs, cu_seqlens, per_sequence, config)
+    reject(not -float("inf") < float(grad_scale) < float("inf"), "grad_scale must be finite")
+    device = _one_device(logits, targets, temperatures, old_logprobs, advantages, mask, ref_logprobs, cu_seqlens)
+    grad = _gradient_output(out, logits)
+    fresh = lambda *shape: torch.empty(shape, device=device, dtype=torch.float32)
+    if tokens == 0:
+        return torch.zeros((), device=device), torch.zeros(7, device=device), fresh(0), grad
+    loss, stats, logprobs = fresh(), fresh(7), fresh(tokens)
+    entropies = fresh(tokens) if config.entropy_coef != 0.0 else None
+    workspace = fresh(query("lfm2_policy_workspace", tokens, sequences, int(cu_seqlens is not None)))
+    _call_on(device, "lfm2_policy_gradient", loss, stats, logprobs, entropies, grad, _row_stride(grad), logits, _row_stride(logits),
+             targets, old_logprobs, advantages, ref_logprobs, mask, cu_seqlens, temperatures, value, workspace, tokens,
+             logits.size(1), sequences, int(per_sequence), *config._arguments(), float(grad_scale), _code(logits.dtype))
+    return loss, stats, logprobs, grad
+
+
 # ----------------------------------------------------------------------------------- measurement
 def hbm_stream_read(buffer: torch.Tensor, sink: torch.Tensor, *, workgroups: int, layout: int = 0) -> int:
     """Launch the loads-only streaming read of `buffer` (`lfm2_hbm_stream_read`); returns the bytes the launch reads.

@@ -23,6 +23,9 @@ extern "C" {
 
 enum { LFM2_OK = 0, LFM2_ERR_ARGUMENT = -1, LFM2_ERR_LAUNCH = -2, LFM2_ERR_UNSUPPORTED = -3 };
 enum { LFM2_DTYPE_BF16 = 0, LFM2_DTYPE_F16 = 1, LFM2_DTYPE_F32 = 2 };
+/* What a policy loss is divided by, and the estimator of its KL term (lfm2_policy_loss). */
+enum { LFM2_MEAN_TOKENS = 0, LFM2_MEAN_SEQUENCES = 1, LFM2_MEAN_SUM = 2 };
+enum { LFM2_KL_K1 = 1, LFM2_KL_K2 = 2, LFM2_KL_K3 = 3 };
 
 const char* lfm2_last_error(void);
 int lfm2_abi_version(void);
@@ -348,6 +351,58 @@ int lfm2_configure_rows(const int64_t* specs, int64_t count, int64_t rows, int32
 /* _record_head of lfm25_session.py:22-31. */
 int lfm2_record_head(const int64_t* ids, const float* probs, int32_t* out_ids, float* out_probs,
                      const int32_t* lengths, const uint8_t* alive, int K, int64_t cap, int64_t B, void* stream);
+
+/* ---------------------------------------------------------------- scoring and the policy loss
+ * No counterparts in the reference's inference path: its scoring converts the logits to fp32 and runs logsumexp and
+ * gather (lfm25_engine.py:1108-1163). */
+
+/* Log-probabilities of given tokens, one pass over the logits: with z = logits[n, :V], T the row's temperature
+ * (temperatures[n], or `temperature` without that array; T <= 0 in the array: 1, as lfm2_sample scores greedy rows),
+ * m = max z and s = sum_v e^{(z_v - m) / T}:
+ *   logprobs[n] = (z_target - m) / T - log s,   entropy[n] = log s - sum_v e^{(z_v - m) / T} (z_v - m) / T / s  (may be NULL),
+ *   stats float[N, 4] = (m, log s, entropy or NaN, 0): what the gradient needs.
+ * Rows are V consecutive elements, row_stride elements apart, at any element alignment.  targets int64[N]: a negative
+ * one takes its row out (zeros, the row is not read); one >= V gives NaN.  A row of -inf only has no distribution:
+ * log-probability -inf, entropy 0.  NaN or +inf in a row makes its results NaN.  Sums in fp32. */
+int lfm2_token_logprobs(float* logprobs, float* entropy, float* stats, const void* logits, int64_t row_stride,
+                        const int64_t* targets, const float* temperatures, float temperature, int64_t N, int64_t V, int dtype,
+                        void* stream);
+/* Its gradient: grad[n, v] = (g ([v = target] - p_v) - h p_v (log p_v + entropy)) / T with g = grad_logprobs[n] and
+ * h = grad_entropy[n] (NULL: none; otherwise `stats` comes from a call with `entropy`), rounded once to the dtype.
+ * Rows taken out, and rows of -inf only, get zeros.  grad may be the logits themselves (same stride). */
+int lfm2_token_logprobs_backward(void* grad, int64_t grad_stride, const void* logits, int64_t row_stride, const int64_t* targets,
+                                 const float* stats, const float* grad_logprobs, const float* grad_entropy,
+                                 const float* temperatures, float temperature, int64_t N, int64_t V, int dtype, void* stream);
+
+/* Clipped policy loss over N packed tokens, sum_t w_t (-gain_t + kl_coef kl_t - entropy_coef entropy_t):
+ *   r = e^{logp - old};  gain = min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A), and max(that, dual_clip A) where A < 0
+ *   if dual_clip > 1 (0: off);  kl, with x = ref - logp: k1 -x, k2 x^2 / 2, k3 e^x - 1 - x (ref NULL: no KL term);
+ *   w = mask / tokens that count (LFM2_MEAN_TOKENS), mask / (tokens that count in the sequence * sequences that have any)
+ *   (LFM2_MEAN_SEQUENCES) or mask (LFM2_MEAN_SUM).
+ * Sequence i is tokens cu_seqlens[i] .. cu_seqlens[i+1] - 1 (int32[S+1], non-decreasing; NULL: one sequence of all N);
+ * tokens behind the last sequence do not count.  mask uint8[N] or NULL.  advantages float[N], or float[S] with
+ * per_sequence.  Nothing that tokens which do not count hold is used.  loss[1]; stats[7] = (sum w (-gain), sum w kl,
+ * sum w entropy, share of tokens cut, mean r, mean of r - 1 - log r, tokens that count); d loss / d logprobs and
+ * d loss / d entropy float[N] (either may be NULL), 0 for tokens that do not count.  Without any token everything is 0.
+ * Whether r is cut is decided on the 64-bit log ratio; sums are 64-bit and joined in a fixed order. */
+int lfm2_policy_loss(float* loss, float* stats, float* grad_logprobs, float* grad_entropy, const float* logprobs, const float* old_logprobs,
+                     const float* advantages, const float* ref_logprobs, const float* entropy, const uint8_t* mask,
+                     const int32_t* cu_seqlens, float* workspace, int64_t N, int64_t S, int per_sequence, int aggregate, int kl,
+                     float clip_low, float clip_high, float dual_clip, float kl_coef, float entropy_coef, void* stream);
+/* 4-byte words of workspace (8-byte aligned) for lfm2_policy_loss and lfm2_policy_gradient. */
+int64_t lfm2_policy_workspace(int64_t N, int64_t S, int has_cu);
+
+/* The same loss straight from the logits, with the gradient of the logits: lfm2_token_logprobs, lfm2_policy_loss and
+ * lfm2_token_logprobs_backward in one pass over the rows that count (a token with a negative target does not).
+ * grad[n, v] = grad_scale * d loss / d logits[n, v], rounded once; rows that do not count get zeros and their logits are
+ * not read.  logprobs float[N] (0 for rows that do not count); entropy float[N], required when entropy_coef != 0.
+ * grad may be the logits themselves (same stride). */
+int lfm2_policy_gradient(float* loss, float* stats, float* logprobs, float* entropy, void* grad, int64_t grad_stride, const void* logits,
+                         int64_t row_stride, const int64_t* targets, const float* old_logprobs, const float* advantages,
+                         const float* ref_logprobs, const uint8_t* mask, const int32_t* cu_seqlens, const float* temperatures,
+                         float temperature, float* workspace, int64_t N, int64_t V, int64_t S, int per_sequence, int aggregate,
+                         int kl, float clip_low, float clip_high, float dual_clip, float kl_coef, float entropy_coef,
+                         float grad_scale, int dtype, void* stream);
 
 /* ---------------------------------------------------------------- measurement */
 

@@ -1,0 +1,468 @@
+"""Log-probabilities of given tokens, the clipped policy loss and their gradients against plain 64-bit forms.
+
+Tolerances count roundings (u = 2^-24 relative each in fp32).  For a row with d_v = (z_v - m) / T:
+  * the exponent of a term takes two roundings of d and the exponential one unit, so a term is off by u (2 |d| + 2); a sum
+    of V of them in the kernel's order (32 values, at most V / 16384 + 12 joins of two roundings) by at most 80 u more; the
+    mean of |d| under p is at most log s + H <= 2 log V.  log s is then off by u (4 log V + 82 + 2 log s);
+  * logp = d_t - log s adds 3 u |d_t|: together u (3 |d_t| + 6 log V + 84);
+  * the entropy is log s - sum(e d) / s: the second sum is a mean of terms |d| with the same relative errors, so its error is
+    that of log s times (1 + mean |d|): u (1 + 2 log V) (6 log V + 84) bounds both;
+  * p_v = 2^{d log2 e - log2 s} is off by u (3 |d| + 6 log V + 90) relative, and a gradient g ([t] - p) - h p (log p + H)
+    by that times |g| p + |h| p (|log p| + H), plus 4 roundings of its terms, plus half a step of the output type.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from climbing_gym_amd import ops as module
+    return module
+
+
+def _rows(n, v, dtype, seed, pad=0, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    wide = (torch.randn(n, v + pad, generator=g) * spread).to(dtype).to(DEV)
+    return wide[:, :v], torch.randint(0, v, (n,), generator=g).to(DEV)
+
+
+def _plain(logits, targets, temperature):
+    """64-bit (logp, H, d, log s, p) from the definition; rows of -inf only give -inf and 0."""
+    t = temperature.double()[:, None] if isinstance(temperature, torch.Tensor) else temperature
+    if isinstance(t, torch.Tensor):
+        t = torch.where(t <= 0, torch.ones_like(t), t)
+    z = logits.double()
+    d = (z - z.amax(1, keepdim=True)) / t
+    e = d.exp()
+    s = e.sum(1, keepdim=True)
+    p = e / s
+    logs = s.log()
+    lp = d.gather(1, targets.clamp(0, logits.size(1) - 1)[:, None])[:, 0] - logs[:, 0]
+    h = logs[:, 0] - torch.where(e > 0, e * d, 0.0).sum(1) / s[:, 0]
+    return lp, h, d, logs, p, t
+
+
+def _check_forward(got_lp, got_h, logits, targets, temperature):
+    lp, h, d, logs, p, _ = _plain(logits, targets, temperature)
+    lv = math.log(max(2, logits.size(1)))
+    live = targets >= 0
+    dt = d.gather(1, targets.clamp_min(0)[:, None])[:, 0].abs()
+    bound = U * (3 * dt + 6 * lv + 84)
+    # (0 - 3.39e38) / 0.5 = -6.8e38 is beyond fp32's largest number, 3.40e38: its fp32 rounding is -inf
+    finite = live & torch.isfinite(lp.float())
+    assert ((got_lp.double() - lp).abs() <= bound)[finite].all(), ((got_lp.double() - lp).abs() / bound)[finite].max()
+    assert torch.equal(got_lp[live & ~finite], lp[live & ~finite].float())
+    assert (got_lp[~live] == 0).all()
+    if got_h is not None:
+        hb = U * (1 + 2 * lv) * (6 * lv + 84)
+        assert ((got_h.double() - h).abs() <= hb)[live].all(), (got_h.double() - h).abs()[live].max()
+        assert (got_h[~live] == 0).all()
+
+
+def _check_grad(got, logits, targets, g, gh, temperature, coefficient_error=0.0):
+    lp, h, d, logs, p, t = _plain(logits, targets, temperature)
+    live = (targets >= 0)[:, None]
+    hot = torch.zeros_like(p).scatter_(1, targets.clamp_min(0)[:, None], 1.0)
+    gg = g.double()[:, None]
+    want = gg * (hot - p)
+    size = gg.abs() * p
+    if gh is not None:
+        logp = torch.where(p > 0, d - logs, 0.0)
+        want = want - gh.double()[:, None] * p * (logp + h[:, None])
+        size = size + gh.double().abs()[:, None] * p * (logp.abs() + h[:, None].abs())
+    want, size = torch.where(live, want / t, 0.0), torch.where(live, (size + gg.abs() * hot) / t, 0.0)
+    lv = math.log(max(2, logits.size(1)))
+    relative = U * (3 * d.clamp_min(-200).abs() + 6 * lv + 90)
+    half = torch.finfo(got.dtype).eps / 2
+    tiny = torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
+    bound = size * (relative + coefficient_error + 4 * U) + half * want.abs() * (1 + 2.0 ** -7) + tiny
+    error = (got.double() - want).abs()
+    assert (error <= bound).all(), (error / bound).max()
+    assert torch.equal(got == got, torch.ones_like(got, dtype=torch.bool))
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16, torch.float32))
+@pytest.mark.parametrize("n, v, pad", ((1, 1, 0), (2, 7, 0), (3, 8, 1), (5, 300, 3), (4, 4097, 0), (3, 8192, 8), (2, 8193, 5),
+                                       (33, 32003, 29), (2, 65536, 0), (1, 131075, 1)))
+def test_logprobs_entropy_and_gradient(ops, dtype, n, v, pad):
+    logits, targets = _rows(n, v, dtype, 7 * v + n, pad)
+    if n > 2:
+        targets[1] = -100
+    gen = torch.Generator().manual_seed(v)
+    g, gh = torch.randn(n, generator=gen).to(DEV), torch.randn(n, generator=gen).to(DEV)
+    per_row = (0.5 + torch.rand(n, generator=gen)).to(DEV)
+    for temperature in (1.0, 0.7, per_row):
+        lp, h, stats = ops.token_logprobs_forward(logits, targets, temperature=temperature, entropy=True)
+        _check_forward(lp, h, logits, targets, temperature)
+        _check_grad(ops.token_logprobs_backward(logits, targets, stats, g, gh, temperature=temperature), logits, targets, g, gh, temperature)
+        lp2, none, stats2 = ops.token_logprobs_forward(logits, targets, temperature=temperature)
+        assert none is None and torch.isnan(stats2[targets >= 0, 2]).all()
+        _check_forward(lp2, None, logits, targets, temperature)
+        _check_grad(ops.token_logprobs_backward(logits, targets, stats2, g, temperature=temperature), logits, targets, g, None, temperature)
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16, torch.float32))
+def test_masked_vocabulary_and_rows_without_a_distribution(ops, dtype):
+    low = torch.finfo(dtype).min
+    logits, targets = _rows(9, 523, dtype, 3)
+    logits = logits.clone()
+    logits[0, ::2] = -math.inf           # half the vocabulary masked
+    logits[1, 5:] = -math.inf            # almost all of it
+    logits[2, 1:] = low                  # the type's lowest value as the mask
+    logits[3] = low                      # nothing else: uniform
+    logits[4] = -math.inf                # no distribution
+    targets[0], targets[1], targets[2], targets[4] = 1, 400, 0, 2
+    logits[5, 17] = math.nan
+    logits[6, 17] = math.inf
+    logits[7, 3] = torch.finfo(dtype).max
+    targets[8] = 523                     # outside the vocabulary
+    g, gh = torch.full((9,), 0.5, device=DEV), torch.full((9,), 0.25, device=DEV)
+    for temperature in (1.0, 0.5):
+        lp, h, stats = ops.token_logprobs_forward(logits, targets, temperature=temperature, entropy=True)
+        keep = torch.tensor([1, 2, 3, 7], device=DEV)
+        assert torch.isfinite(lp[torch.tensor([0, 2, 3], device=DEV)]).logical_or(lp[torch.tensor([0, 2, 3], device=DEV)] == -math.inf).all()
+        _check_forward(lp[keep], h[keep], logits[keep], targets[keep], temperature)
+        assert lp[1] == -math.inf and lp[4] == -math.inf and h[4] == 0
+        assert torch.isnan(lp[5]) and torch.isnan(lp[6]) and torch.isnan(lp[8])
+        grad = ops.token_logprobs_backward(logits, targets, stats, g, gh, temperature=temperature)
+        _check_grad(grad[keep], logits[keep], targets[keep], g[keep], gh[keep], temperature)
+        assert (grad[4] == 0).all()
+        assert torch.isnan(grad[5]).all() and torch.isnan(grad[6]).all() and torch.isnan(grad[8]).all()
+        assert (grad[0, 2::2] == 0).all()
+
+
+def test_greedy_rows_are_scored_at_temperature_one(ops):
+    logits, targets = _rows(4, 1000, torch.bfloat16, 5)
+    t = torch.tensor([0.0, -1.0, 1.0, 0.5], device=DEV)
+    lp, _, _ = ops.token_logprobs_forward(logits, targets, temperature=t)
+    _check_forward(lp, None, logits, targets, t)
+
+
+def test_log_probability_of_a_draw_equals_the_samplers(ops):
+    logits, _ = _rows(16, 65536, torch.bfloat16, 6)
+    tempered = torch.empty(16, device=DEV)
+    tokens, raw = ops.sample_logits(logits.contiguous(), temperature=0.7, seed=3, step=1, return_logprobs=True, sampling_logprobs=tempered)
+    torch.testing.assert_close(ops.token_logprobs(logits, tokens), raw, atol=4e-5, rtol=0)
+    torch.testing.assert_close(ops.token_logprobs(logits, tokens, temperature=0.7), tempered, atol=4e-5, rtol=0)
+
+
+def test_gradient_in_place_and_into_a_padded_matrix(ops):
+    logits, targets = _rows(6, 1001, torch.bfloat16, 8, pad=7)
+    g = torch.randn(6, generator=torch.Generator().manual_seed(1)).to(DEV)
+    _, _, stats = ops.token_logprobs_forward(logits, targets)
+    want = ops.token_logprobs_backward(logits, targets, stats, g)
+    wide = torch.full((6, 1010), 9.0, device=DEV, dtype=torch.bfloat16)
+    got = ops.token_logprobs_backward(logits, targets, stats, g, out=wide[:, 3:1004])
+    assert torch.equal(got, want) and (wide[:, :3] == 9).all() and (wide[:, 1004:] == 9).all()
+    parent = torch.full((6, 1008), 5.0, device=DEV, dtype=torch.bfloat16)
+    parent[:, :1001] = logits
+    inplace = parent[:, :1001]
+    assert ops.token_logprobs_backward(inplace, targets, stats, g, out=inplace) is inplace
+    assert torch.equal(inplace, want) and (parent[:, 1001:] == 5).all()
+    with pytest.raises(ValueError, match="share no storage"):
+        ops.token_logprobs_backward(parent[:, :1001], targets, stats, g, out=parent[:, 1:1002])
+
+
+def test_autograd_of_the_log_probabilities(ops):
+    logits, targets = _rows(5, 777, torch.float32, 9)
+    leaf = logits.clone().requires_grad_()
+    lp, h = ops.token_logprobs(leaf * 1.0, targets, temperature=0.8, entropy=True)
+    (lp.sum() - 0.3 * h.mean()).backward()     # a broadcast gradient arrives with stride 0
+    _check_grad(leaf.grad, logits, targets, torch.ones(5, device=DEV), torch.full((5,), -0.06, device=DEV), 0.8, 2 * U)
+    leaf2 = logits.clone().requires_grad_()
+    _, h2 = ops.token_logprobs(leaf2, targets, entropy=True)
+    h2.sum().backward()                        # the log-probabilities have no gradient at all
+    _check_grad(leaf2.grad, logits, targets, torch.zeros(5, device=DEV), torch.ones(5, device=DEV), 1.0)
+    # differences: (f(z + e) - f(z - e)) / 2e in 64 bits of the plain form, against the kernel's gradient
+    direction = torch.randn(5, 777, generator=torch.Generator().manual_seed(2)).to(DEV).double()
+    f = lambda z: (lambda r: r[0].sum() - 0.3 * r[1].mean())(_plain(z, targets, 0.8))
+    e = 1e-5
+    slope = (f(logits.double() + e * direction) - f(logits.double() - e * direction)) / (2 * e)
+    assert abs((leaf.grad.double() * direction).sum() - slope) <= 1e-4 * (1 + abs(slope))
+
+
+# --------------------------------------------------------------------------------------------- the loss
+def _definition(lp, old, a, mask, ref, h, bounds, cfg):
+    """The loss from its definition in 64 bits on the CPU; `a` per token; differentiable in lp and h."""
+    live = mask.clone()
+    n = len(lp)
+    seq = torch.full((n,), -1)
+    for i, (s, e) in enumerate(zip(bounds[:-1], bounds[1:])):
+        seq[s:e] = i
+    live &= seq >= 0
+    idx = live.nonzero()[:, 0]
+    if len(idx) == 0:
+        return lp.sum() * 0, torch.zeros(7, dtype=torch.float64)
+    l, o, adv, sq = lp[idx], old[idx], a[idx], seq[idx]
+    if cfg.aggregate == "token":
+        w = torch.full((len(idx),), 1.0 / len(idx), dtype=torch.float64)
+    elif cfg.aggregate == "sum":
+        w = torch.ones(len(idx), dtype=torch.float64)
+    else:
+        c = torch.bincount(sq, minlength=len(bounds) - 1)
+        w = 1.0 / (c[sq].double() * (c > 0).sum())
+    r = (l - o).exp()
+    clipped = r.clamp(1 - cfg.clip_low, 1 + cfg.clip_high) * adv
+    gain = torch.minimum(r * adv, clipped)
+    cut = clipped < r * adv
+    if cfg.dual_clip:
+        cut = cut | ((adv < 0) & (cfg.dual_clip * adv > gain))
+        gain = torch.where(adv < 0, torch.maximum(gain, cfg.dual_clip * adv), gain)
+    kl = torch.zeros_like(l)
+    if ref is not None:
+        x = ref[idx] - l
+        kl = {"k1": -x, "k2": x * x / 2, "k3": torch.expm1(x) - x}[cfg.kl]
+    policy, klm = -(w * gain).sum(), (w * kl).sum()
+    hm = (w * h[idx]).sum() if h is not None else torch.zeros((), dtype=torch.float64)
+    d = (l - o).detach()
+    stats = torch.stack([policy.detach(), klm.detach(), hm.detach(), cut.double().mean(), r.detach().mean(),
+                         (torch.expm1(d) - d).mean(), torch.tensor(float(len(idx)), dtype=torch.float64)])
+    return policy + cfg.kl_coef * klm - cfg.entropy_coef * hm, stats
+
+
+def _tokens(n, seed):
+    g = torch.Generator().manual_seed(seed)
+    old = -2 * torch.rand(n, generator=g) ** 2
+    return (old + 0.3 * torch.randn(n, generator=g), old, torch.randn(n, generator=g), torch.rand(n, generator=g) < 0.7,
+            old + 0.3 * torch.randn(n, generator=g), torch.rand(n, generator=g))
+
+
+# sums are 64-bit; each term is off by its own fp32 roundings: expf 2 u, the products with the advantage and the weight
+# u each, the KL series 4 u of its value: 12 u of the sum of the terms' sizes covers loss, statistics and gradients
+def _compare_loss(got, want_loss, want_stats, want_grad, sizes):
+    loss, stats, grad = got
+    assert abs(loss.double().cpu() - want_loss) <= 12 * U * sizes
+    assert (abs(stats.double().cpu() - want_stats) <= 12 * U * (sizes + want_stats.abs() + 1)).all()
+    assert stats[6].item() == want_stats[6]
+    error = (grad.double().cpu() - want_grad).abs()
+    assert (error <= 12 * U * (want_grad.abs() + want_grad.abs().max() * 4)).all(), error.max()
+
+
+BOUNDS = {"one": lambda n: [0, n], "empty ones": lambda n: [0, 0, n // 3, n // 3, n // 3, n, n],
+          "padded tail": lambda n: [0, n // 2, n - n // 5],
+          "single tokens": lambda n: list(range(min(n, 300))) + [n]}
+
+
+@pytest.mark.parametrize("n", (1, 2, 63, 1000, 4096, 4097, 70001))
+@pytest.mark.parametrize("aggregate", ("token", "sequence", "sum"))
+@pytest.mark.parametrize("layout", (None, *BOUNDS))
+def test_policy_loss_and_gradient(ops, n, aggregate, layout):
+    lp, old, a, mask, ref, h = _tokens(n, n)
+    bounds = BOUNDS[layout](n) if layout else [0, n]
+    variants = [dict(), dict(kl="k1", kl_coef=0.1), dict(kl="k2", kl_coef=0.1, dual_clip=1.5), dict(kl_coef=0.2, entropy_coef=0.05)]
+    for number, kw in enumerate(variants):
+        cfg = ops.PolicyLossConfig(clip_low=0.2, clip_high=0.3, aggregate=aggregate, **kw)
+        use_mask, per_sequence = number % 2 == 1, number >= 2 and layout is not None
+        adv = torch.randn(len(bounds) - 1, generator=torch.Generator().manual_seed(3)) if per_sequence else a
+        token_adv = a.double().clone()
+        if per_sequence:
+            for i, (s, e) in enumerate(zip(bounds[:-1], bounds[1:])):
+                token_adv[s:e] = adv[i].double()
+        m = mask if use_mask else torch.ones(n, dtype=torch.bool)
+        x, hh = lp.double().requires_grad_(), h.double().requires_grad_()
+        want, stats = _definition(x, old.double(), token_adv, m, ref.double() if cfg.kl_coef else None,
+                                  hh if cfg.entropy_coef else None, bounds, cfg)
+        want_g, want_h = torch.autograd.grad(want, (x, hh), allow_unused=True)
+        dev = lambda t: None if t is None else t.to(DEV)
+        got = ops.policy_loss_forward(dev(lp), dev(old), dev(adv), mask=dev(mask) if use_mask else None,
+                                      ref_logprobs=dev(ref) if cfg.kl_coef else None, entropy=dev(h) if cfg.entropy_coef else None,
+                                      cu_seqlens=torch.tensor(bounds, dtype=torch.int32).to(DEV) if layout else None,
+                                      per_sequence=per_sequence, config=cfg)
+        sizes = (want_g.abs().sum() + stats[:3].abs().sum() + 1).item() * (n if aggregate == "sum" else 1)
+        _compare_loss(got[:3], want.detach(), stats, want_g, sizes)
+        if cfg.entropy_coef:
+            want_h = torch.zeros(n, dtype=torch.float64) if want_h is None else want_h     # no token counted
+            torch.testing.assert_close(got[3].double().cpu(), want_h, rtol=4 * U, atol=0)
+
+
+def test_tokens_that_do_not_count_may_hold_anything(ops):
+    n = 5000
+    lp, old, a, mask, ref, h = _tokens(n, 4)
+    cfg = ops.PolicyLossConfig(kl_coef=0.1, entropy_coef=0.1)
+    call = lambda *t: ops.policy_loss_forward(*[x.to(DEV) for x in t[:3]], mask=mask.to(DEV), ref_logprobs=t[3].to(DEV), entropy=t[4].to(DEV), config=cfg)
+    want = call(lp, old, a, ref, h)
+    dirty = [x.clone() for x in (lp, old, a, ref, h)]
+    for i, x in enumerate(dirty):
+        x[~mask] = (math.nan, math.inf, -math.inf)[i % 3]
+    for got, expected in zip(call(*dirty), want):
+        assert torch.equal(got, expected)
+
+
+def test_without_a_token_that_counts_everything_is_zero(ops):
+    for n in (0, 3, 6000):
+        lp, old, a, _, ref, _ = _tokens(n, 5)
+        for aggregate in ("token", "sequence", "sum"):
+            loss, stats, grad, _ = ops.policy_loss_forward(lp.to(DEV), old.to(DEV), a.to(DEV), mask=torch.zeros(n, dtype=torch.bool, device=DEV),
+                                                           cu_seqlens=torch.tensor([0, n // 2, n], dtype=torch.int32, device=DEV),
+                                                           config=ops.PolicyLossConfig(aggregate=aggregate))
+            assert loss.item() == 0 and (stats == 0).all() and grad.shape == (n,) and (grad == 0).all()
+
+
+def test_ratios_at_the_border(ops):
+    """One unit in the last place on either side of the cut decides between the full slope and none."""
+    high, low = math.log1p(0.25), math.log1p(-0.25)
+    near = lambda x: [torch.nextafter(torch.tensor(x), torch.tensor(s)).item() for s in (-9.0, 9.0)] + [torch.tensor(x).item()]
+    d = torch.tensor(near(high) + near(low) + near(high) + near(low))
+    a = torch.tensor([1.0] * 6 + [-1.0] * 6)
+    _, _, grad, _ = ops.policy_loss_forward(d.to(DEV), torch.zeros(12, device=DEV), a.to(DEV), config=ops.PolicyLossConfig(clip_low=0.25, clip_high=0.25, aggregate="sum"))
+    cut = ((a > 0) & (d.double() > high)) | ((a < 0) & (d.double() < low))
+    assert torch.equal(grad.cpu() == 0, cut)
+
+
+def test_policy_loss_is_the_same_on_every_call(ops):
+    lp, old, a, mask, ref, _ = [x.to(DEV) for x in _tokens(300000, 6)]
+    cfg = ops.PolicyLossConfig(kl_coef=0.1)
+    first = ops.policy_loss_forward(lp, old, a, mask=mask, ref_logprobs=ref, config=cfg)
+    for _ in range(3):
+        for x, y in zip(first[:3], ops.policy_loss_forward(lp, old, a, mask=mask, ref_logprobs=ref, config=cfg)[:3]):
+            assert torch.equal(x, y)
+
+
+# --------------------------------------------------------------------------------------------- the run together
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("bounds, v", (([0, 1], 5), ([0, 9, 9, 40], 1003), ([0, 20, 30], 4096), ([0, 3, 50, 60], 32003)))
+@pytest.mark.parametrize("entropy_coef", (0.0, 0.02))
+def test_scoring_loss_and_gradient_together(ops, dtype, bounds, v, entropy_coef):
+    """token_logprobs -> policy_loss -> backward, and policy_gradient, against each other and the 64-bit definition."""
+    n = bounds[-1]
+    logits, targets = _rows(n, v, dtype, v)
+    g = torch.Generator().manual_seed(v)
+    now = _plain(logits, targets, 0.9)[0].float().cpu()
+    old, ref = now + 0.3 * torch.randn(n, generator=g), now + 0.3 * torch.randn(n, generator=g)
+    adv, mask = torch.randn(len(bounds) - 1, generator=g), torch.rand(n, generator=g) < 0.8
+    if n > 4:
+        targets[3] = -1
+    live = mask & (targets.cpu() >= 0)
+    cfg = ops.PolicyLossConfig(clip_low=0.2, clip_high=0.3, kl_coef=0.1, entropy_coef=entropy_coef, aggregate="sequence")
+    dev = lambda t: t.to(DEV)
+    kw = dict(mask=dev(mask), ref_logprobs=dev(ref), cu_seqlens=dev(torch.tensor(bounds, dtype=torch.int32)), per_sequence=True, config=cfg)
+    loss, stats, logprobs, grad = ops.policy_gradient(logits, targets, dev(old), dev(adv), temperature=0.9, **kw)
+    assert (logprobs[~dev(live)] == 0).all() and (grad[~dev(live)] == 0).all()
+
+    leaf = logits.clone().requires_grad_()
+    out = ops.token_logprobs(leaf, targets, temperature=0.9, entropy=entropy_coef != 0)
+    lp, h = out if entropy_coef else (out, None)
+    kw2 = {**kw, "mask": dev(live)}
+    loss2, stats2 = ops.policy_loss(lp, dev(old), dev(adv), entropy=h, **kw2)
+    (2.0 * loss2).backward()
+    torch.testing.assert_close(loss, loss2.detach(), rtol=4 * U, atol=4 * U)
+    torch.testing.assert_close(stats, stats2, rtol=8 * U, atol=8 * U)
+    # The two routes may sum a row in different orders: their log-probabilities then differ by twice the bound on one, D,
+    # the slope w (-A r + kl (1 - e^x)) by w (|A| r + kl e^x) D (r and e^x are their own derivatives), the gradient by that
+    # times ([t] + p) / T, p itself by 2 D p, and each side rounds once to the type.
+    _, _, d, _, p, _ = _plain(logits, targets, 0.9)
+    hot = torch.zeros_like(p).scatter_(1, targets.clamp_min(0)[:, None], 1.0)
+    dt = d.gather(1, targets.clamp_min(0)[:, None])[:, 0].abs()
+    apart = 2 * U * (3 * dt + 6 * math.log(v + 1) + 90)
+    lengths = torch.tensor(bounds).diff()
+    counted = torch.stack([live[s:e].sum() for s, e in zip(bounds[:-1], bounds[1:])]).clamp_min(1)
+    weight = dev((1.0 / (counted.double() * (counted > 0).sum())).repeat_interleave(lengths))
+    ratio, other = (logprobs - dev(old)).double().exp(), (dev(ref) - logprobs).double().exp()
+    size = weight * (dev(adv).double().repeat_interleave(dev(lengths)).abs() * ratio + 0.1 * (1 + other))
+    bound = 2 * (size * apart)[:, None] * (hot + p) / 0.9 + 4 * (size * apart)[:, None] * p / 0.9
+    if entropy_coef:   # w c p (log p + H): |log p + H| <= |d| + 2 log V, and D more for each of its parts
+        bound = bound + 2 * entropy_coef * (weight * apart)[:, None] * p * (2 * d.abs() + 4 * math.log(v + 1) + 2) / 0.9
+    step = torch.finfo(dtype).eps
+    bound = bound + 2 * step * grad.double().abs() + 4 * torch.finfo(dtype).smallest_normal * step
+    error = (leaf.grad.double() - 2 * grad.double()).abs()
+    assert (error <= bound)[dev(live)].all(), (error / bound)[dev(live)].max()
+    assert (leaf.grad[~dev(live)] == 0).all()
+
+    # the kernel's own log-probabilities in the definition: the loss and its slope, then the logits' gradient
+    token_adv = torch.zeros(n, dtype=torch.float64)
+    for i, (s, e) in enumerate(zip(bounds[:-1], bounds[1:])):
+        token_adv[s:e] = adv[i].double()
+    x = logprobs.double().cpu().requires_grad_()
+    hh = _plain(logits, targets, 0.9)[1].cpu().requires_grad_()
+    want, want_stats = _definition(x, old.double(), token_adv, live, ref.double(), hh if entropy_coef else None, bounds, cfg)
+    want_g, want_h = torch.autograd.grad(want, (x, hh), allow_unused=True)
+    _check_forward(torch.where(dev(live), logprobs, 0), None, logits, torch.where(dev(live), targets, -1), 0.9)
+    assert abs(loss.double().cpu() - want) <= 40 * U * (1 + want_stats[:3].abs().sum()) * (1 + 6 * math.log(v + 1))
+    _check_grad(grad, logits, torch.where(dev(live), targets, -1), dev(want_g.float()),
+                dev(want_h.float()) if entropy_coef else None, 0.9, 32 * U)
+
+
+def test_policy_gradient_scale_in_place_and_padded_rows(ops):
+    logits, targets = _rows(30, 515, torch.bfloat16, 12, pad=5)
+    old = ops.token_logprobs(logits, targets) + 0.05
+    adv = torch.randn(30, generator=torch.Generator().manual_seed(3)).to(DEV)
+    cu = torch.tensor([0, 10, 24], dtype=torch.int32, device=DEV)   # six rows behind the last sequence
+    kw = dict(cu_seqlens=cu, config=ops.PolicyLossConfig())
+    _, stats, lp, grad = ops.policy_gradient(logits, targets, old, adv, **kw)
+    assert stats[6].item() == 24 and (grad[24:] == 0).all() and (lp[24:] == 0).all()
+    _, _, _, scaled = ops.policy_gradient(logits, targets, old, adv, grad_scale=1024.0, **kw)
+    assert torch.equal(scaled.float(), 1024.0 * grad.float())       # a power of two only moves exponents
+    copy = logits.clone()
+    assert ops.policy_gradient(copy, targets, old, adv, out=copy, **kw)[3] is copy
+    assert torch.equal(copy, grad)
+
+
+def test_policy_calls_replay_inside_a_graph(ops):
+    logits, targets = _rows(64, 4099, torch.bfloat16, 13)
+    old = ops.token_logprobs(logits, targets).clone()
+    adv = torch.randn(64, generator=torch.Generator().manual_seed(4)).to(DEV)
+    mask = torch.ones(64, dtype=torch.bool, device=DEV)
+    cfg = ops.PolicyLossConfig(kl_coef=0.1, aggregate="sequence")
+    cu = torch.tensor([0, 30, 64], dtype=torch.int32, device=DEV)
+
+    def step():
+        lp, _, stats = ops.token_logprobs_forward(logits, targets)
+        loss, _, g, _ = ops.policy_loss_forward(lp, old, adv, mask=mask, ref_logprobs=old, cu_seqlens=cu, config=cfg)
+        grad = ops.token_logprobs_backward(logits, targets, stats, g)
+        fused = ops.policy_gradient(logits, targets, old, adv, mask=mask, ref_logprobs=old, cu_seqlens=cu, config=cfg)
+        return (loss, g, grad, *fused)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+        leaf = logits.detach().float().requires_grad_()
+        with pytest.raises(RuntimeError, match="graph capture"):
+            ops.token_logprobs(leaf, targets)
+        with pytest.raises(RuntimeError, match="graph capture"):
+            ops.policy_loss(old.detach().requires_grad_(), old, adv)
+    for seed in range(3):
+        gen = torch.Generator().manual_seed(seed)
+        logits.copy_((torch.randn(64, 4099, generator=gen) * 2).bfloat16())
+        mask.copy_(torch.rand(64, generator=gen) < 0.6)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(held, step()):
+            assert torch.equal(got, want)
+
+
+def test_calls_on_a_side_stream(ops):
+    logits, targets = _rows(40, 8000, torch.bfloat16, 14)
+    want = ops.token_logprobs(logits, targets)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.token_logprobs(logits, targets)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def test_refusals_on_the_device(ops):
+    logits, targets = _rows(4, 50, torch.bfloat16, 15)
+    row = torch.zeros(4, device=DEV)
+    for bad in (lambda: ops.token_logprobs(logits.t(), targets), lambda: ops.token_logprobs(logits[:, ::2], targets),
+                lambda: ops.token_logprobs(logits[:1].expand(4, 50), targets), lambda: ops.token_logprobs(logits, targets.int()),
+                lambda: ops.token_logprobs(logits, targets[:3]), lambda: ops.token_logprobs(logits, targets, temperature=0.0),
+                lambda: ops.token_logprobs(logits, targets, temperature=row.double()), lambda: ops.token_logprobs(logits.double(), targets),
+                lambda: ops.token_logprobs(logits[:, :0], targets), lambda: ops.token_logprobs(logits, targets.cpu()),
+                lambda: ops.token_logprobs_backward(logits, targets, torch.zeros(4, 3, device=DEV), row),
+                lambda: ops.token_logprobs_backward(logits, targets, torch.zeros(4, 4, device=DEV), row.expand(4).double()),
+                lambda: ops.policy_gradient(logits, targets, row, row[:2]), lambda: ops.policy_gradient(logits, targets, row, row, grad_scale=math.inf),
+                lambda: ops.policy_gradient(logits, targets, row, row, out=torch.zeros(4, 50, device=DEV)),
+                lambda: ops.policy_loss(row, row.cpu(), row)):
+        with pytest.raises(ValueError):
+            bad()
+    empty = ops.token_logprobs(logits[:0], targets[:0])
+    assert empty.shape == (0,)
