@@ -50,6 +50,8 @@ _SIGNATURES = {
     "lfm2_decode_attention": "pppppppppp" "lipp" "liiillllfiippp",
     "lfm2_decode_schedule": "pppp" "lp",
     "lfm2_decode_begin": "pppppppp" "lp",
+    "lfm2_shared_schedule": "ppppppp" "llliii" "p",
+    "lfm2_shared_attention": "pppppppp" "lip" "liiilllll" "fiip",
     "lfm2_prefill_attention": "ppppp" "lliiifip",
     "lfm2_build_token_map": "ppp" "llp",
     "lfm2_gather_inputs": "ppppppp" "lp",
@@ -80,6 +82,8 @@ _INT64_RESULT = {
     "lfm2_bf16_gemm_workspace": "lll",
     "lfm2_decode_attention_workspace": "liil",
     "lfm2_decode_schedule_size": "ll",
+    "lfm2_shared_schedule_size": "lliii",
+    "lfm2_shared_attention_workspace": "lliii",
     "lfm2_policy_workspace": "lli",
     "lfm2_timestamp_rate_khz": "",
 }

@@ -5,7 +5,7 @@ import os
 import subprocess
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = ("elementwise.hip", "gemm.hip", "attention.hip", "sampling.hip", "policy.hip")
+SOURCES = ("elementwise.hip", "gemm.hip", "attention.hip", "sampling.hip", "shared_attention.hip", "policy.hip")
 LIBRARY = os.path.join(HERE, "liblfm2_hip.so")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-ffp-contract=off", "-Wno-unused",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

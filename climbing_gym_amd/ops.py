@@ -39,6 +39,26 @@ def _check(*tensors):
         reject(not t.is_contiguous(), "HIP kernels require contiguous tensors")
 
 
+def _one_device(*tensors):
+    """The device all given tensors (None: left out) live on; the launch goes to that device's current stream."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        reject(not t.is_cuda, "HIP kernels require GPU tensors")
+        reject(device is not None and t.device != device, "all tensors of a call live on one device")
+        device = t.device
+    return device
+
+
+def _call_on(device, name: str, *args) -> None:
+    if device.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
+
+
 # ----------------------------------------------------------------------------------- embedding / norms
 def embedding(tokens: torch.Tensor, table: torch.Tensor) -> torch.Tensor:
     """F.embedding of lfm25_cuda.py:134 for int64 token ids."""
@@ -524,6 +544,95 @@ def decode(q, k, v, k_cache, v_cache, k_scales, v_scales, positions, *, active=N
                   window=window, schedule=schedule)
 
 
+@dataclass(frozen=True)
+class SharedPrefix:
+    """Rows of a decode batch in groups that share the first part of their history (the completions of one prompt): group g
+    is rows starts[g] .. starts[g+1] - 1, and the first lengths[g] positions of those rows are the ones slot slots[g] holds
+    (with a block table: the ones table row slots[g] names).  All int32 on the device; slots[g] < 0 shares nothing."""
+    starts: torch.Tensor
+    slots: torch.Tensor
+    lengths: torch.Tensor
+
+    def check(self):
+        for name, t in (("starts", self.starts), ("slots", self.slots), ("lengths", self.lengths)):
+            reject(t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous(), f"prefix {name} must be a contiguous int32 vector")
+        reject(self.slots.numel() == 0 or self.starts.numel() != self.slots.numel() + 1 or self.lengths.numel() != self.slots.numel(),
+               "a shared prefix needs one slot and one length per group and one bound more")
+
+
+def _check_batch_rows(positions, active, slot_ids):
+    rows = positions.numel()
+    reject(positions.dtype != torch.int32 or positions.ndim != 1 or rows == 0 or not positions.is_contiguous(),
+           "positions must be a contiguous int32 vector")
+    reject(active is not None and (active.dtype not in (torch.bool, torch.uint8) or active.shape != (rows,) or not active.is_contiguous()),
+           "active must be a bool mask, one per row")
+    reject(slot_ids is not None and (slot_ids.dtype != torch.int32 or slot_ids.shape != (rows,) or not slot_ids.is_contiguous()),
+           "slot_ids must be int32, one per row")
+    return rows
+
+
+def shared_schedule(positions, prefix: SharedPrefix, active=None, slot_ids=None, *, capacity: int, query_heads: int,
+                    kv_heads: int, head_dim: int):
+    """Work list of `attend_shared` for the rows' current lengths: built once per decode step (it depends on nothing a layer
+    computes) and passed to every layer's call."""
+    rows = _check_batch_rows(positions, active, slot_ids)
+    prefix.check()
+    device = _one_device(positions, prefix.starts, prefix.slots, prefix.lengths, active, slot_ids)
+    reject(query_heads <= 0 or kv_heads <= 0 or query_heads % kv_heads, "query heads must be a multiple of the KV heads")
+    size = query("lfm2_shared_schedule_size", rows, int(capacity), query_heads, kv_heads, head_dim)
+    schedule = torch.empty(max(size, 4), device=device, dtype=torch.int32)
+    _call_on(device, "lfm2_shared_schedule", schedule, positions, active, slot_ids, prefix.starts, prefix.slots, prefix.lengths,
+             rows, prefix.slots.numel(), int(capacity), query_heads, kv_heads, head_dim)
+    return schedule
+
+
+def attend_shared(q, k_cache, v_cache, k_scales, v_scales, positions, prefix: SharedPrefix, *, active=None, scale=None,
+                  slot_ids=None, block_table=None, page=16, schedule=None, quantized=False):
+    """`attend` for rows that share the first part of their history in groups: the same result as with a copy of the prefix
+    in every row's slot, with one reading of the prefix per group and no copies (lfm25_engine.py:761 forks a prompt's cache
+    once per completion).  Positions below `prefix.lengths[g]` are read from slot `prefix.slots[g]`, the others from the
+    row's own slot, where the decode step appends them at their usual positions.  `schedule`: `shared_schedule` of the same
+    positions, prefix, mask and shapes (built here when None).  Slots or pages outside the cache give NaN rows."""
+    reject(q.ndim != 4 or q.size(1) != 1 or q.dtype not in (torch.bfloat16, torch.float16), "queries must be bf16 or fp16 [rows, 1, heads, dim]")
+    rows, _, query_heads, dim = q.shape
+    reject(_check_batch_rows(positions, active, slot_ids) != rows, "positions must have one entry per row")
+    prefix.check()
+    device = _one_device(q, k_cache, v_cache, k_scales, v_scales, positions, prefix.starts, prefix.slots, prefix.lengths, active,
+                         slot_ids, block_table, schedule)
+    reject(not q.is_contiguous(), "HIP kernels require contiguous tensors")
+    strides = _cache_strides(k_cache)
+    pools, _, heads, width = k_cache.shape
+    fp8 = k_scales is not None
+    reject(width != dim or v_cache.shape != k_cache.shape or _cache_strides(v_cache) != strides, "key and value caches must match each other and the head dim")
+    reject(k_cache.dtype != (FP8 if fp8 else q.dtype) or v_cache.dtype != k_cache.dtype, "the history is e4m3 with scales, or of the queries' type without")
+    reject(heads == 0 or query_heads % heads, "query heads must be a multiple of the KV heads")
+    reject(fp8 != (v_scales is not None), "an e4m3 history needs both scale tensors")
+    if fp8:
+        for s in (k_scales, v_scales):
+            reject(s.dtype != torch.float32 or s.shape != k_cache.shape[:3]
+                   or any(n > 1 and a * dim != b for n, a, b in zip(s.shape, s.stride(), strides)),
+                   "scales must be fp32, laid out as the cache with one value per token and head")
+    if block_table is None:
+        capacity = k_cache.size(1)
+    else:
+        reject(block_table.dtype != torch.int32 or block_table.ndim != 2 or block_table.size(0) != rows or not block_table.is_contiguous(),
+               "block_table must be a contiguous int32 [rows, blocks] tensor")
+        reject(page != k_cache.size(1), "page must be the pages' size")
+        capacity = block_table.size(1) * page
+    if schedule is None:
+        schedule = shared_schedule(positions, prefix, active, slot_ids, capacity=capacity, query_heads=query_heads, kv_heads=heads, head_dim=dim)
+    else:
+        reject(schedule.dtype != torch.int32 or not schedule.is_contiguous()
+               or schedule.numel() < query("lfm2_shared_schedule_size", rows, capacity, query_heads, heads, dim),
+               "schedule must come from shared_schedule for this batch")
+    ws = torch.empty(query("lfm2_shared_attention_workspace", rows, capacity, query_heads, heads, dim), device=device, dtype=torch.float32)
+    out = torch.empty_like(q)
+    _call_on(device, "lfm2_shared_attention", out, q, k_cache, v_cache, k_scales, v_scales, schedule, block_table,
+             0 if block_table is None else block_table.size(1), int(page), ws, rows, query_heads, heads, dim, capacity, pools, *strides,
+             float(scale if scale is not None else dim ** -0.5), int(fp8), _code(q.dtype))
+    return quantize_rows(out.view(rows, query_heads * dim)) if quantized else out
+
+
 def prefill_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float | None = None):
     """Varlen causal GQA attention (flash_attn_func of lfm25_engine.py:1415-1417 on a packed batch):
     q [tokens, QH, D], k/v [tokens, KH, D], cu_seqlens int32."""
@@ -692,26 +801,6 @@ def record_head(ids, probs, out_ids, out_probs, lengths, alive, k: int, cap: int
 
 
 # ----------------------------------------------------------------------------------- scoring and policy loss
-def _one_device(*tensors):
-    """The device all given tensors (None: left out) live on; the launch goes to that device's current stream."""
-    device = None
-    for t in tensors:
-        if t is None:
-            continue
-        reject(not t.is_cuda, "HIP kernels require GPU tensors")
-        reject(device is not None and t.device != device, "all tensors of a call live on one device")
-        device = t.device
-    return device
-
-
-def _call_on(device, name: str, *args) -> None:
-    if device.index == torch.cuda.current_device():
-        call(name, *args)
-    else:
-        with torch.cuda.device(device):
-            call(name, *args)
-
-
 def _check_logits(logits, targets, temperature):
     reject(logits.ndim != 2 or not logits.is_cuda or logits.dtype not in DTYPE_CODE,
            "scoring requires a 2D GPU BF16/FP16/FP32 logits tensor")

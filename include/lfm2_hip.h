@@ -257,6 +257,30 @@ int64_t lfm2_decode_schedule_size(int64_t B, int64_t capacity);
 int lfm2_decode_begin(int32_t* schedule, int32_t* positions_out, int64_t* tokens_out, uint8_t* mask_out, int32_t* lengths,
                       const int64_t* input, const uint8_t* active, const int32_t* slots, int64_t B, void* stream);
 
+/* Decode attention of a batch whose rows share histories in groups (completions of one prompt).  Group g is rows
+ * starts[g] .. starts[g+1] - 1 (int32[groups+1], non-decreasing, within [0, B]; a row outside every group shares nothing).
+ * The history of a row of group g at positions < prefix_lengths[g] is that of slot prefix_slots[g] (of block-table row
+ * prefix_slots[g] with a block table), at the positions from there on its own slot's (its own table row's), and it attends
+ * over [0, positions[b]] as lfm2_decode_attention does: the result is what that call gives when every row's slot holds a
+ * copy of the prefix, without the copies and with one reading of the prefix per group.  prefix_slots[g] < 0: no shared part.
+ * Inactive rows, rows with slot_ids[b] < 0 and rows of length 0 produce zeros; positions beyond the capacity are cut to it.
+ * Slots and pages outside the cache, bounds out of order and a work list of another batch give NaN rows.
+ *
+ * lfm2_shared_schedule builds the work list of one decode step, int32[lfm2_shared_schedule_size()], 16-byte aligned: it
+ * depends on the lengths and groups only, so a step's attention layers share it.  At most 4096 rows and 4096 groups. */
+int lfm2_shared_schedule(int32_t* schedule, const int32_t* positions, const uint8_t* active, const int32_t* slot_ids,
+                         const int32_t* starts, const int32_t* prefix_slots, const int32_t* prefix_lengths, int64_t B,
+                         int64_t groups, int64_t capacity, int QH, int KH, int D, void* stream);
+int64_t lfm2_shared_schedule_size(int64_t B, int64_t capacity, int QH, int KH, int D);
+/* q, out [B,QH,D] bf16 or fp16; history in that type, or e4m3 with fp32 scales (kv_fp8; scales at the element's offset / D);
+ * `pools` slots, or pages with block_table int32[B,max_blocks] (then c0 is the page stride); D in {32, 64, 128};
+ * workspace: lfm2_shared_attention_workspace() floats. */
+int lfm2_shared_attention(void* out, const void* q, const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,
+                          const int32_t* schedule, const int32_t* block_table, int64_t max_blocks, int page, float* workspace,
+                          int64_t B, int QH, int KH, int D, int64_t capacity, int64_t pools, int64_t c0, int64_t c1, int64_t c2,
+                          float scale, int kv_fp8, int dtype, void* stream);
+int64_t lfm2_shared_attention_workspace(int64_t B, int64_t capacity, int QH, int KH, int D);
+
 /* flash_attn_func(causal=True) of lfm25_engine.py:1415-1417 in varlen form: q [T,QH,D], k,v [T,KH,D]
  * packed by cu_seqlens int32[nseq+1]; out [T,QH,D]. */
 int lfm2_prefill_attention(void* out, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,

@@ -71,3 +71,36 @@ def test_c_boundary_refuses(library):
         assert loss(**kw) == -1 and text in message(), kw
     assert library.lfm2_policy_workspace(0, 1, 0) == 0
     assert library.lfm2_policy_workspace(1, 1, 1) >= 15
+
+
+def test_shared_attention_refuses_at_the_c_boundary(library):
+    buffer = ctypes.create_string_buffer(4096 + 16)
+    p = (ctypes.addressof(buffer) + 15) // 16 * 16
+    message = lambda: library.lfm2_last_error().decode()
+    def schedule(b=4, groups=1, capacity=64, qh=8, kh=2, d=64, at=p, starts=p):
+        return library.lfm2_shared_schedule(at, p, None, None, starts, p, p, b, groups, capacity, qh, kh, d, None)
+    for kw, text in ((dict(b=0), "empty"), (dict(b=5000), "rows"), (dict(groups=0), "groups"), (dict(groups=5000), "groups"), (dict(capacity=0), "empty"),
+                     (dict(capacity=1 << 29), "positions"), (dict(kh=3), "divisible"), (dict(d=80), "head_dim"), (dict(at=p + 4), "unaligned"),
+                     (dict(starts=None), "bounds"), (dict(qh=2048), "query heads")):
+        assert schedule(**kw) == -1 and text in message(), (kw, message())
+    def attend(b=4, d=64, q=p, c1=64, fp8=0, table=None, page=16, blocks=0, pools=4, dtype=0, scales=None, ws=p):
+        return library.lfm2_shared_attention(p, q, p, p, scales, scales, p, table, blocks, page, ws, b, 8, 2, d, 64, pools, 64 * 128, c1, 64, 0.125, fp8, dtype, None)
+    for kw, status, text in ((dict(b=0), -1, "empty"), (dict(q=p + 2), -1, "aligned"), (dict(c1=65), -1, "strides"), (dict(c1=16, fp8=1, scales=p), -1, "strides"),
+                             (dict(fp8=1), -1, "scales"), (dict(table=p, blocks=3), -1, "page"), (dict(pools=0), -1, "cache"),
+                             (dict(dtype=2), -3, "dtype"), (dict(ws=None), -1, "null")):
+        assert attend(**kw) == status and text in message(), (kw, message())
+    assert library.lfm2_shared_schedule_size(0, 64, 8, 2, 64) == 0 and library.lfm2_shared_attention_workspace(4, 64, 8, 3, 64) == 0
+    assert library.lfm2_shared_schedule_size(4, 64, 8, 2, 64) >= 16 + 4 * 4 + 8 * 8
+
+
+def test_binding_signatures_match_the_header():
+    """Kinds and number of the arguments the binding passes, against the declarations."""
+    import os
+    import re
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "lfm2_hip.h")).read()
+    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    kind = lambda arg: "p" if "*" in arg else "l" if "int64_t" in arg else "f" if "float" in arg else "i"
+    declared = {name: "".join(kind(a) for a in args.split(",") if a.strip() not in ("", "void"))
+                for name, args in re.findall(r"\b(?:int|int64_t)\s+(lfm2_\w+)\s*\(([^)]*)\)", text)}
+    for name, signature in {**_lib._SIGNATURES, **_lib._INT64_RESULT}.items():
+        assert declared[name] == signature, name

@@ -1,0 +1,303 @@
+"""Decode attention over shared prefixes against the definition in 64 bits: every row's history put together from the
+prefix slot and its own, softmax, weighted sum.
+
+Tolerance of an output o = sum p v / sum p, with A = sum p |v| / sum p:
+  * probabilities are rounded to the type of the second product, h relative (bf16 2^-8, also for every e4m3 history; fp16
+    2^-11), once in the numerator only: h A; below fp16's normal range the step is 2^-24, so n tokens add n 2^-25 max |v|
+    at most (the largest probability is at least 1 in the kernel's units);
+  * a score is a sum of D products in fp32: off by (D + 4) 2^-24 sum |q k| scale, the exponential's argument and result
+    by |s| 2^-23 and 2^-23, together d; numerator and denominator: 2 d A; sums of n terms in fp32 and the joining of the
+    partial results: 2^-18 A covers lengths up to the longest here;
+  * the output's own rounding: half a step of it.
+"""
+import math
+import random
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+FP8 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from climbing_gym_amd import ops as module
+    return module
+
+
+class Batch:
+    """Caches, queries and groups; unused positions hold NaN.  `groups`: (row count, prefix length, slot offset or None)."""
+
+    def __init__(self, groups, own, *, heads=(8, 2), dim=64, dtype=torch.bfloat16, fp8=False, page=0, loose=0, seed=0, token_major=False,
+                 slot_ids=False, active=None, scale=None):
+        self.ops_kw = {}
+        g = torch.Generator().manual_seed(seed)
+        rng = random.Random(seed)
+        (self.qh, self.kh), self.dim, self.dtype, self.fp8, self.page = heads, dim, dtype, fp8, page
+        self.starts, self.prefix_rows, self.prefix_len = [0], [], []
+        rows = sum(n for n, *_ in groups) + loose
+        self.rows = rows
+        self.shared, self.leader = [0] * rows, list(range(rows))
+        at = 0
+        for n, length, leader in groups:
+            self.starts.append(at + n)
+            lead = -1 if leader is None else at + leader
+            self.prefix_rows.append(lead)
+            self.prefix_len.append(length)
+            for b in range(at, at + n):
+                if lead >= 0:
+                    self.shared[b], self.leader[b] = length, lead
+            at += n
+        self.lens = [max(0, self.shared[b] + own[b % len(own)]) for b in range(rows)]
+        self.active = active
+        cap = max(max(self.lens), max(self.prefix_len, default=1), 1) + 5
+        spare = 3
+        slots = rows + spare
+        self.map = list(range(rows))
+        if slot_ids:
+            self.map = rng.sample(range(slots), rows)
+        make = lambda: torch.randn(slots, cap, self.kh, dim, generator=g).to(dtype)
+        self.k, self.v = make(), make()
+        self.q = (1.5 * torch.randn(rows, 1, self.qh, dim, generator=g)).to(dtype)
+        self.scale = dim ** -0.5 if scale is None else scale
+        held = [0] * slots     # positions of a slot anybody may read
+        first = [cap] * slots
+        for b in range(rows):
+            s = self.map[b]
+            held[s], first[s] = max(held[s], self.lens[b]), min(first[s], self.shared[b])
+            lead = self.map[self.leader[b]]
+            if self.shared[b]:
+                held[lead], first[lead] = max(held[lead], min(self.shared[b], max(self.lens))), 0
+        for t in (self.k, self.v):
+            for s in range(slots):
+                t[s, held[s]:] = math.nan
+                t[s, :first[s]] = math.nan
+        if fp8:
+            self.ks, self.vs, self.k, self.v = None, None, *[t for t in (self.k, self.v)]
+            codes = []
+            for t in (self.k, self.v):
+                s = (t.float().abs().amax(-1) / 448).clamp_min(1e-12)
+                codes.append(((t.float() / s[..., None]).to(FP8), s))
+            (self.k, self.ks), (self.v, self.vs) = codes
+        else:
+            self.ks = self.vs = None
+        self.table = None
+        dense = lambda t: t if t is None or token_major else t.to(DEV).transpose(1, 2).contiguous().transpose(1, 2)
+        if page:
+            blocks = -(-cap // page)
+            pools = slots * blocks + 2
+            order = rng.sample(range(pools), slots * blocks)
+            table = torch.tensor(order, dtype=torch.int32).view(slots, blocks)
+            def paged(t):
+                if t is None:
+                    return None
+                pad = torch.full((slots, blocks * page, *t.shape[2:]), math.nan).to(t.dtype)
+                bits = lambda x: x.view(torch.uint8) if x.element_size() == 1 else x
+                bits(pad)[:, :cap] = bits(t)
+                out = torch.full((pools, page, *t.shape[2:]), math.nan).to(t.dtype)
+                bits(out)[table.long().view(-1)] = bits(pad).view(slots * blocks, page, *t.shape[2:])
+                return out.to(DEV)
+            self.dk, self.dv, self.dks, self.dvs = [paged(t) for t in (self.k, self.v, self.ks, self.vs)]
+            self.table = table[self.map].contiguous().to(DEV)
+        else:
+            self.dk, self.dv, self.dks, self.dvs = [None if t is None else dense(t).to(DEV) for t in (self.k, self.v, self.ks, self.vs)]
+        ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+        self.positions = ints([n - 1 for n in self.lens])
+        where = lambda lead: lead if lead < 0 else lead if page else self.map[lead]
+        self.prefix_args = (ints(self.starts), ints([where(r) for r in self.prefix_rows]), ints(self.prefix_len))
+        self.slot_ids = ints(self.map) if slot_ids and not page else None
+        self.mask = None if active is None else torch.tensor(active, device=DEV)
+
+    def run(self, ops, **kw):
+        args = dict(active=self.mask, scale=self.scale, slot_ids=self.slot_ids, block_table=self.table, page=self.page or 16)
+        return ops.attend_shared(self.q.to(DEV), self.dk, self.dv, self.dks, self.dvs, self.positions, ops.SharedPrefix(*self.prefix_args),
+                                 **{**args, **kw})
+
+    def expected(self):
+        """(outputs, bounds) in 64 bits."""
+        wide = lambda t, s: t.double() if s is None else t.float().double() * s.double()[..., None]
+        k, v = wide(self.k, self.ks), wide(self.v, self.vs)
+        out = torch.zeros(self.rows, 1, self.qh, self.dim, dtype=torch.float64)
+        bound = torch.full_like(out, 1e-30)
+        per = self.qh // self.kh
+        u = 2.0 ** -24
+        half = torch.finfo(self.dtype).eps / 2
+        h = 2.0 ** -8 if self.fp8 or self.dtype == torch.bfloat16 else 2.0 ** -11
+        for b in range(self.rows):
+            n = self.lens[b]
+            if n <= 0 or (self.active is not None and not self.active[b]):
+                continue
+            lead, own, cut = self.map[self.leader[b]], self.map[b], min(self.shared[b], n)
+            kk, vv = [torch.cat((t[lead, :cut], t[own, cut:n])).permute(1, 0, 2) for t in (k, v)]   # [kh, n, dim]
+            q = self.q[b, 0].double().view(self.kh, per, self.dim)
+            s = self.scale * (q @ kk.transpose(1, 2))
+            size = self.scale * (q.abs() @ kk.abs().transpose(1, 2))
+            p = torch.softmax(s, -1)
+            out[b, 0] = (p @ vv).reshape(self.qh, self.dim)
+            d = ((self.dim + 4) * u * size + 2 * u * (s.abs() * 1.5 + 1)).amax(-1, keepdim=True)
+            spread = p @ vv.abs()
+            limit = (h + 2 * d + 2.0 ** -18) * spread + half * out[b, 0].abs().view(self.kh, per, self.dim)
+            if self.dtype == torch.float16 and not self.fp8:
+                limit = limit + n * 2.0 ** -25 * vv.abs().amax()
+            bound[b, 0] = limit.reshape(self.qh, self.dim) + 1e-30
+        return out, bound
+
+    def check(self, ops, **kw):
+        got = self.run(ops, **kw)
+        want, bound = self.expected()
+        error = (got.double().cpu() - want).abs()
+        assert got.dtype == self.dtype and got.shape == self.q.shape
+        assert (error <= bound).all(), ((error / bound).nan_to_num(nan=math.inf).max(), (error <= bound).float().mean())
+        return got
+
+
+GROUPS = [(4, 100, 0), (1, 33, 0), (7, 260, 3), (3, 0, 0), (2, 64, None), (16, 513, 0)]
+OWN = (1, 2, 31, 32, 33, 64, 127, 128, 129, 200, 300)
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("fp8", (False, True))
+@pytest.mark.parametrize("dim", (32, 64, 128))
+@pytest.mark.parametrize("heads", ((8, 2), (4, 4), (24, 2), (6, 2), (40, 1)))
+def test_types_and_head_layouts(ops, dtype, fp8, dim, heads):
+    Batch(GROUPS, OWN, heads=heads, dim=dim, dtype=dtype, fp8=fp8, loose=2, seed=dim + heads[0]).check(ops)
+
+
+@pytest.mark.parametrize("fp8", (False, True))
+@pytest.mark.parametrize("dim", (32, 64, 128))
+@pytest.mark.parametrize("page", (1, 16, 24, 64))
+def test_paged_histories(ops, fp8, dim, page):
+    Batch(GROUPS, OWN, heads=(8, 2), dim=dim, fp8=fp8, page=page, loose=1, seed=page).check(ops)
+
+
+@pytest.mark.parametrize("length", (1, 2, 31, 32, 33, 63, 64, 127, 128, 129, 1000, 2500))
+def test_lengths(ops, length):
+    Batch([(5, length, 0)], (1, 40), heads=(8, 2), seed=length).check(ops)
+    Batch([(5, 7, 0)], (length, 1), heads=(8, 2), seed=length).check(ops)
+    Batch([(1, length, 0)], (length,), heads=(4, 2), dim=128, fp8=True, seed=length).check(ops)
+
+
+@pytest.mark.parametrize("rows", (1, 3, 4, 5, 8, 9, 15, 16, 17, 40))
+@pytest.mark.parametrize("fp8", (False, True))
+def test_group_sizes(ops, rows, fp8):
+    Batch([(rows, 150, rows - 1), (1, 5, 0), (rows, 90, 0)], (1, 17, 50), heads=(8, 2), fp8=fp8, seed=rows).check(ops)
+
+
+def test_rows_that_sit_out_and_rows_shorter_than_the_prefix(ops):
+    groups = [(4, 100, 0), (3, 300, 0), (5, 40, 1)]
+    active = [True, False, True, True] + [False] * 3 + [True, True, False, True, True]
+    own = (3, 5, -60, -99, 1, 1, 1, -40, 2, 8, -1, 0)     # lengths within the prefix, and 0
+    for fp8 in (False, True):
+        got = Batch(groups, own, active=active, fp8=fp8, seed=3).check(ops)
+        assert (got[1] == 0).all() and (got[4:7] == 0).all() and (got[7] == 0).all()
+
+
+def test_slot_maps_token_major_caches_and_other_scales(ops):
+    Batch(GROUPS, OWN, slot_ids=True, seed=5).check(ops)
+    Batch(GROUPS, OWN, token_major=True, fp8=True, seed=6).check(ops)
+    Batch(GROUPS, OWN, token_major=True, dim=128, seed=7, scale=0.3).check(ops)
+    batch = Batch(GROUPS, OWN, slot_ids=True, seed=8)
+    batch.slot_ids[2] = -1       # padding row
+    got = batch.run(ops)
+    assert (got[2] == 0).all()
+
+
+def test_equals_attend_on_copied_prefixes(ops):
+    for fp8 in (False, True):
+        batch = Batch([(6, 200, 0), (4, 77, 0)], (1, 9, 100, 150), fp8=fp8, seed=9)
+        shared = batch.run(ops)
+        copies = [t.clone() for t in (batch.dk, batch.dv)] + [None if t is None else t.clone() for t in (batch.dks, batch.dvs)]
+        for b in range(batch.rows):
+            for t in copies:
+                if t is not None:
+                    raw = t.view(torch.uint8) if t.element_size() == 1 else t
+                    raw[b, :batch.shared[b]] = raw[batch.leader[b], :batch.shared[b]].clone()
+        plain = ops.attend(batch.q.to(DEV), *copies, batch.positions)
+        want, bound = batch.expected()
+        assert ((shared.double() - plain.double()).abs().cpu() <= 2 * bound).all()
+
+
+def test_one_schedule_serves_every_layer_and_quantised_rows(ops):
+    batch = Batch(GROUPS, OWN, fp8=True, seed=10)
+    prefix = ops.SharedPrefix(*batch.prefix_args)
+    schedule = ops.shared_schedule(batch.positions, prefix, batch.mask, capacity=batch.dk.size(1), query_heads=8, kv_heads=2, head_dim=64)
+    first = batch.check(ops, schedule=schedule)
+    assert torch.equal(first, batch.check(ops, schedule=schedule))
+    q, scales = batch.run(ops, schedule=schedule, quantized=True)
+    want_q, want_scales = ops.quantize_rows(first.view(batch.rows, -1))
+    assert torch.equal(q.view(torch.uint8), want_q.view(torch.uint8)) and torch.equal(scales, want_scales)
+
+
+def test_large_scores_keep_their_order(ops):
+    """Scores of several hundred: only the largest survives, wherever it is."""
+    batch = Batch([(4, 300, 0)], (50, 100), seed=11, scale=20.0)
+    batch.check(ops)
+
+
+def test_many_rows_and_a_long_history(ops):
+    Batch([(40, 700, 0)] * 3 + [(1, 9, 0)] * 70, (1, 5, 64), heads=(4, 1), seed=12).check(ops)
+    Batch([(2, 20000, 0)], (3, 9000), heads=(4, 1), seed=13, fp8=True).check(ops)
+
+
+def test_bad_slots_pages_bounds_and_foreign_schedules_give_nan(ops):
+    batch = Batch([(2, 100, 0), (2, 50, 0)], (9, 40), seed=14)
+    starts, slots, lengths = batch.prefix_args
+    run = lambda *prefix, **kw: ops.attend_shared(batch.q.to(DEV), batch.dk, batch.dv, None, None, batch.positions, ops.SharedPrefix(*prefix), **kw)
+    bad = slots.clone()
+    bad[1] = batch.dk.size(0)
+    got = run(starts, bad, lengths)
+    assert torch.isfinite(got[:2]).all() and torch.isnan(got[2:]).all()
+    got = run(starts, slots, lengths, slot_ids=torch.tensor([0, 10000, 2, 3], dtype=torch.int32, device=DEV))
+    assert torch.isnan(got[1]).all() and torch.isfinite(got[[0, 2, 3]]).all()
+    assert torch.isnan(run(torch.tensor([0, 4, 2], dtype=torch.int32, device=DEV), slots, lengths)).all()
+    other = ops.shared_schedule(batch.positions, ops.SharedPrefix(*batch.prefix_args), capacity=batch.dk.size(1) + 1000, query_heads=8, kv_heads=2, head_dim=64)
+    assert torch.isnan(run(starts, slots, lengths, schedule=other)).all()
+    paged = Batch([(2, 100, 0), (2, 50, 0)], (9, 40), page=16, seed=15)
+    paged.table[1, 6] = 1 << 20      # row 1's own part
+    paged.table[2, 0] = -1           # the second group's prefix
+    got = paged.run(ops)
+    assert torch.isfinite(got[0]).all() and torch.isnan(got[1:]).all()
+
+
+def test_replays_inside_a_graph_with_other_lengths(ops):
+    batch = Batch([(6, 200, 0), (4, 77, 0)], (150,), fp8=True, seed=16)
+    prefix = ops.SharedPrefix(*batch.prefix_args)
+    q = batch.q.to(DEV)
+    call = lambda: ops.attend_shared(q, batch.dk, batch.dv, batch.dks, batch.dvs, batch.positions, prefix)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call()
+    for own in (150, 3, 64, 1):
+        batch.lens = [s + own for s in batch.shared]
+        batch.positions.copy_(torch.tensor([n - 1 for n in batch.lens], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, call())
+        want, bound = batch.expected()
+        assert ((held.double().cpu() - want).abs() <= bound).all()
+
+
+def test_refusals(ops):
+    batch = Batch([(2, 100, 0), (2, 50, 0)], (9, 40), seed=17)
+    prefix = ops.SharedPrefix(*batch.prefix_args)
+    q, k, v, pos = batch.q.to(DEV), batch.dk, batch.dv, batch.positions
+    for bad in (lambda: ops.attend_shared(q[:, 0], k, v, None, None, pos, prefix), lambda: ops.attend_shared(q.float(), k, v, None, None, pos, prefix),
+                lambda: ops.attend_shared(q.half(), k, v, None, None, pos, prefix), lambda: ops.attend_shared(q, k, v[:, :-1], None, None, pos, prefix),
+                lambda: ops.attend_shared(q, k, v, None, None, pos.long(), prefix), lambda: ops.attend_shared(q, k, v, None, None, pos[:2], prefix),
+                lambda: ops.attend_shared(q, k, v, batch.mask, k, pos, prefix),
+                lambda: ops.attend_shared(q, k, v, None, None, pos, ops.SharedPrefix(prefix.starts[1:], prefix.slots, prefix.lengths)),
+                lambda: ops.attend_shared(q, k, v, None, None, pos, ops.SharedPrefix(prefix.starts, prefix.slots.long(), prefix.lengths)),
+                lambda: ops.attend_shared(q, k, v, None, None, pos, prefix, active=torch.ones(3, dtype=torch.bool, device=DEV)),
+                lambda: ops.attend_shared(q, k, v, None, None, pos, prefix, slot_ids=pos.long()),
+                lambda: ops.attend_shared(q, k, v, None, None, pos, prefix, schedule=pos),
+                lambda: ops.attend_shared(q, k, v, None, None, pos, prefix, block_table=pos.view(4, 1), page=16),
+                lambda: ops.attend_shared(q.cpu(), k, v, None, None, pos, prefix),
+                lambda: ops.shared_schedule(pos, prefix, capacity=0, query_heads=8, kv_heads=2, head_dim=64),
+                lambda: ops.shared_schedule(pos, prefix, capacity=64, query_heads=8, kv_heads=3, head_dim=64),
+                lambda: ops.shared_schedule(pos, prefix, capacity=64, query_heads=8, kv_heads=2, head_dim=80)):
+        with pytest.raises(ValueError):
+            bad()
