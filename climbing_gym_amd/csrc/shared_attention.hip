@@ -9,34 +9,42 @@
 namespace {
 
 constexpr float kInf = __builtin_huge_valf();
-constexpr int kTile = 32;                 // history tokens per wave and step
-constexpr int kGrain = 4 * kTile;         // chunks are whole steps of the workgroup's four waves
+constexpr int kStep = 32;                 // history tokens that meet 16 queries at a time
+constexpr int kShareTile = 4 * kStep;     // tokens a workgroup stages at a time of a part that a group shares
+constexpr int kGrain = 128;               // chunks are multiples of this
 constexpr int kMaxRows = 4096;            // rows and groups the work list holds
-constexpr int kSplitSlots = 2048;         // partial results beyond one per row, for the shared and for the own part
-constexpr int kSharedItems = 1024;        // workgroup items the shared parts are cut into, if their length allows ...
-constexpr int kOwnItems = 2048;           // ... and the rows' own parts
-
-// Queries of one item: a tile of the (row, head) pairs of a group that use one KV head.
-constexpr int query_tile(int D) { return D <= 64 ? 64 : 32; }
+constexpr int kSplitSlots = 2048;         // partial results beyond one per row and part, for each of the two chunk sizes
+constexpr int kQueryTile = 64;            // queries of an item that a group shares: its (row, head) pairs of one KV head
+constexpr int kQueryBlock = 16;           // queries of the other items
+constexpr int kTurn = 256;                // workgroups, one per CU
+constexpr int kSharedBlocks = 2 * kTurn, kOtherBlocks = 3 * kTurn;
+constexpr int kSharedItems = 512;      // items the shared parts are cut into, if their length allows ...
+constexpr int kOwnItems = 2048;         // ... and the others
+constexpr int kWaveTokens = 128;      // up to this many tokens an item is one wave's
 
 // ---- the work list (int32), built once per decode step and used by every attention layer
-//   header: what the list was built for, number of records, number of shared records
+//   header: what the list was built for, number of records of each of the three kinds of item
 //   one record per row: first partial result, shared chunks, own chunks, length (0: sits out)
-//   one record per item: first row, rows, query tile, first partial result's offset within a row, first token, end token,
-//   slot or table row that holds them, 1 for a shared part
-enum { kHRecords, kHRows, kHCapacity, kHQueryHeads, kHKvHeads, kHDim, kHeader = 16 };
+//   one record per item, kind after kind: first row, rows, query tile, place of the partial result among the row's, first
+//   token, end token, slot or table row that holds them, 1 for a part that a group shares
+// A group with more queries than a block has its shared part cut into "shared" items, of a workgroup and up to 64 queries.
+// Everything else (rows' own parts, the shared parts of smaller groups) becomes items of one block of queries: a workgroup's
+// ("long"), or a wave's ("short") where the part has at most kWaveTokens tokens.
+enum { kHShared, kHLong, kHShort, kHRows, kHCapacity, kHQueryHeads, kHKvHeads, kHDim, kHeader = 16 };
 constexpr int kRowInts = 4, kRecordInts = 8;
 
 struct SlotBounds { int64_t slots, records; };
-// Upper bounds of the partial results and of the items of a batch, from what the host knows.
-SlotBounds slot_bounds(int64_t B, int64_t capacity, int G, int D) {
+// Upper bounds of the partial results and of the items of a batch, from what the host knows.  A row has at most
+// ceil(capacity / kGrain) shared and as many own chunks; a chunk size is at least 1 / kSplitSlots of the tokens it cuts (with
+// multiplicity, the shared ones counted once per row), so each of the two sizes makes at most kSplitSlots chunks plus one
+// per part, and a row has two parts.  An item covers at least one row's queries, or a tile of them.
+SlotBounds slot_bounds(int64_t B, int64_t capacity, int G) {
   const int64_t per_row = (capacity + kGrain - 1) / kGrain;
   const int64_t half = B * per_row < B + kSplitSlots ? B * per_row : B + kSplitSlots;
-  const int64_t tile = query_tile(D), tiles = (G + tile - 1) / tile;
-  return SlotBounds{2 * half, half * (2 * tiles + 1)};
+  return SlotBounds{2 * half, 2 * half * ((G + kQueryBlock - 1) / kQueryBlock)};
 }
-int64_t schedule_ints(int64_t B, int64_t capacity, int G, int D) {
-  return kHeader + kRowInts * B + kRecordInts * slot_bounds(B, capacity, G, D).records;
+int64_t schedule_ints(int64_t B, int64_t capacity, int G) {
+  return kHeader + kRowInts * B + kRecordInts * slot_bounds(B, capacity, G).records;
 }
 
 struct ScheduleArgs {
@@ -77,7 +85,7 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
   __shared__ int starts[kMaxRows + 1], length[kMaxRows], extent[kMaxRows];
   __shared__ int scratch[16];
   __shared__ float fscratch[16];
-  const int tid = threadIdx.x, G = a.QH / a.KH, tile = query_tile(a.D);
+  const int tid = threadIdx.x, G = a.QH / a.KH;
   const int capacity = (int)a.capacity;
   for (int g = tid; g <= a.groups; g += 1024) {
     const int s = a.starts[g];
@@ -117,82 +125,108 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
   }
   __syncthreads();
   // chunk sizes: enough items to fill the chip, no more partial results than the workspace holds
-  float row_tokens = 0.f, own_tokens = 0.f, work = 0.f;
+  auto queries = [&](int g) { return (starts[g + 1] - starts[g]) * G; };
+  auto wide = [&](int g) { return queries(g) > kQueryBlock; };
+  const int own_tiles = (G + kQueryBlock - 1) / kQueryBlock;
+  float wide_tokens = 0.f, other_tokens = 0.f, wide_work = 0.f, other_work = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int b = tid * PER + i;
     if (b >= a.B) continue;
-    if (group[i] >= 0) row_tokens += (float)extent[group[i]];
-    if (length[b] > shared[i]) own_tokens += (float)(length[b] - shared[i]);
+    if (group[i] >= 0) (wide(group[i]) ? wide_tokens : other_tokens) += (float)extent[group[i]];
+    if (length[b] > shared[i]) {
+      other_tokens += (float)(length[b] - shared[i]);
+      other_work += (float)(length[b] - shared[i]) * (float)own_tiles;
+    }
   }
-  auto group_tiles = [&](int g) {   // query tiles of a group whose rows share anything
-    const int rows = starts[g + 1] - starts[g];
-    return extent[g] > 0 && rows > 0 ? (rows * G + tile - 1) / tile : 0;
-  };
-  for (int g = tid; g < a.groups; g += 1024) work += (float)extent[g] * (float)group_tiles(g);
-  row_tokens = sum_1024(row_tokens, fscratch);
-  own_tokens = sum_1024(own_tokens, fscratch);
-  work = sum_1024(work, fscratch);
-  const int own_tiles = (G + tile - 1) / tile;
-  auto chunk_of = [&](float slots_tokens, float item_tokens, int items) {
-    // one more step than the quotient: the sums are rounded
-    const float need = fmaxf(slots_tokens / (float)kSplitSlots, item_tokens * (float)a.KH / (float)items);
+  for (int g = tid; g < a.groups; g += 1024) {
+    if (wide(g)) wide_work += (float)extent[g] * (float)((queries(g) + kQueryTile - 1) / kQueryTile);
+    else other_work += (float)extent[g];
+  }
+  wide_tokens = sum_1024(wide_tokens, fscratch);
+  other_tokens = sum_1024(other_tokens, fscratch);
+  wide_work = sum_1024(wide_work, fscratch);
+  other_work = sum_1024(other_work, fscratch);
+  auto chunk_of = [&](float tokens, float work, int items) {
+    // a little more than the quotient: the sums are rounded
+    const float need = fmaxf(tokens / (float)kSplitSlots, work * (float)a.KH / (float)items);
     return round_up((int)fminf(need * 1.0001f, 1.0e9f) + 1, kGrain);
   };
-  const int shared_chunk = chunk_of(row_tokens, work, kSharedItems);
-  const int own_chunk = chunk_of(own_tokens, own_tokens * (float)own_tiles, kOwnItems);
-  // places: partial results of every row, then the records of the shared parts and of the own parts
-  int slots = 0, own_records = 0;
+  const int wide_chunk = chunk_of(wide_tokens, wide_work, kSharedItems);
+  const int other_chunk = chunk_of(other_tokens, other_work, kOwnItems);
+  // a part's chunks, and its records by kind (0 shared, 1 long, 2 short)
+  struct Part { int chunk, chunks, records, kind; };
+  auto shared_part = [&](int g) {
+    Part p;
+    p.chunk = wide(g) ? wide_chunk : other_chunk;
+    p.chunks = (extent[g] + p.chunk - 1) / p.chunk;
+    p.records = p.chunks * (wide(g) ? (queries(g) + kQueryTile - 1) / kQueryTile : 1);
+    p.kind = wide(g) ? 0 : extent[g] > kWaveTokens ? 1 : 2;
+    return p;
+  };
+  auto own_part = [&](int tokens) {
+    Part p;
+    p.chunk = other_chunk;
+    p.chunks = tokens > 0 ? (tokens + p.chunk - 1) / p.chunk : 0;
+    p.records = p.chunks * own_tiles;
+    p.kind = tokens > kWaveTokens ? 1 : 2;
+    return p;
+  };
+  // places: partial results of every row, then the records, kind after kind
+  int slots = 0, mine[3] = {0, 0, 0};
   int np[PER], ns[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int b = tid * PER + i;
     np[i] = ns[i] = 0;
-    if (b >= a.B) continue;
-    if (group[i] >= 0) np[i] = (extent[group[i]] + shared_chunk - 1) / shared_chunk;
-    if (length[b] > shared[i]) ns[i] = (length[b] - shared[i] + own_chunk - 1) / own_chunk;
-    slots += np[i] + ns[i];
-    own_records += ns[i] * own_tiles;
+    if (b < a.B) {
+      if (group[i] >= 0) np[i] = shared_part(group[i]).chunks;
+      const Part own = own_part(length[b] - shared[i]);
+      ns[i] = own.chunks;
+      slots += np[i] + ns[i];
+      mine[1] += own.kind == 1 ? own.records : 0;
+      mine[2] += own.kind == 2 ? own.records : 0;
+    }
+    if (b < a.groups) {   // the same numbers once more, for groups
+      const Part part = shared_part(b);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) mine[k] += part.kind == k ? part.records : 0;
+    }
   }
-  int total, shared_total, own_total;
+  int total, totals[3], at[3], before = 0;
   int slot = scan_1024(slots, scratch, &total);
-  int shared_records = 0;
-  for (int i = 0; i < PER; ++i) {
-    const int g = tid * PER + i;
-    if (g < a.groups) shared_records += (extent[g] + shared_chunk - 1) / shared_chunk * group_tiles(g);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    at[k] = before + scan_1024(mine[k], scratch, &totals[k]);
+    before += totals[k];
   }
-  int record = scan_1024(shared_records, scratch, &shared_total);
-  int own_record = shared_total + scan_1024(own_records, scratch, &own_total);
   int32_t* const records = a.schedule + kHeader + kRowInts * a.B;
-  auto put = [&](int at, int row, int rows, int qt, int offset, int t0, int t1, int source, int is_shared) {
-    i32x4* r = reinterpret_cast<i32x4*>(records + (int64_t)kRecordInts * at);
-    r[0] = i32x4{row, rows, qt, offset};
-    r[1] = i32x4{t0, t1, source, is_shared};
+  auto put = [&](const Part& part, int row, int rows, int tiles, int offset, int t0, int end, int source, int is_shared) {
+    int& place = part.kind == 0 ? at[0] : part.kind == 1 ? at[1] : at[2];
+    for (int c = 0; c < part.chunks; ++c)
+      for (int qt = 0; qt < tiles; ++qt) {
+        i32x4* r = reinterpret_cast<i32x4*>(records + (int64_t)kRecordInts * place++);
+        r[0] = i32x4{row, rows, qt, offset + c};
+        r[1] = i32x4{t0 + c * part.chunk, min(t0 + (c + 1) * part.chunk, end), source, is_shared};
+      }
   };
-  for (int i = 0; i < PER; ++i) {
-    const int g = tid * PER + i;
-    if (g >= a.groups) break;
-    const int tiles = group_tiles(g);
-    for (int t0 = 0, c = 0; tiles > 0 && t0 < extent[g]; t0 += shared_chunk, ++c)
-      for (int qt = 0; qt < tiles; ++qt)
-        put(record++, starts[g], starts[g + 1] - starts[g], qt, c, t0, min(t0 + shared_chunk, extent[g]), a.prefix_slots[g], 1);
-  }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int b = tid * PER + i;
-    if (b >= a.B) continue;
-    int32_t* r = a.schedule + kHeader + kRowInts * b;
-    r[0] = slot; r[1] = np[i]; r[2] = ns[i]; r[3] = length[b];
-    slot += np[i] + ns[i];
-    const int source = a.slot_ids ? a.slot_ids[b] : b;
-    for (int c = 0; c < ns[i]; ++c)
-      for (int qt = 0; qt < own_tiles; ++qt) {
-        const int t0 = shared[i] + c * own_chunk;
-        put(own_record++, b, 1, qt, np[i] + c, t0, min(t0 + own_chunk, length[b]), source, 0);
-      }
+    if (b < a.B) {
+      *reinterpret_cast<i32x4*>(a.schedule + kHeader + kRowInts * b) = i32x4{slot, np[i], ns[i], length[b]};
+      slot += np[i] + ns[i];
+      put(own_part(length[b] - shared[i]), b, 1, own_tiles, np[i], shared[i], length[b], a.slot_ids ? a.slot_ids[b] : b, 0);
+    }
+    if (b < a.groups) {
+      const Part part = shared_part(b);
+      if (part.chunks) put(part, starts[b], starts[b + 1] - starts[b], part.records / part.chunks, 0, 0, extent[b], a.prefix_slots[b], 1);
+    }
   }
   if (tid == 0) {
-    a.schedule[kHRecords] = shared_total + own_total;
+    a.schedule[kHShared] = totals[0];
+    a.schedule[kHLong] = totals[1];
+    a.schedule[kHShort] = totals[2];
     a.schedule[kHRows] = a.B;
     a.schedule[kHCapacity] = capacity;
     a.schedule[kHQueryHeads] = a.QH;
@@ -227,6 +261,14 @@ template <> __device__ __forceinline__ f16x8 widen8<_Float16>(int lo, int hi) {
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// Lanes of a wave exchange values through LDS: the hardware keeps a wave's LDS accesses in order, and this keeps the
+// compiler from moving or reusing them across the exchange.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 struct SharedArgs {
   void* out;
   const void *q, *kc, *vc;
@@ -234,7 +276,7 @@ struct SharedArgs {
   const int32_t *schedule, *table;
   float *acc, *m, *l;          // partial results: [slot][query head][D], [slot][query head] twice
   int64_t c0, c1, c2, max_blocks, pools, sources;   // pools: slots or pages; sources: slots or table rows
-  int page, page_shift, B, QH, KH, G, capacity;
+  int page, page_shift, B, QH, KH, G, capacity, shared_blocks, other_blocks;
   float scale_log2e;
 };
 __device__ __forceinline__ bool list_fits(const SharedArgs& a, int D) {
@@ -242,279 +284,465 @@ __device__ __forceinline__ bool list_fits(const SharedArgs& a, int D) {
   return s[kHRows] == a.B && s[kHCapacity] == a.capacity && s[kHQueryHeads] == a.QH && s[kHKvHeads] == a.KH && s[kHDim] == D;
 }
 
-// One item: MT * 16 queries against tokens [t0, t1) of one KV head.  The four waves take the tokens in tiles of 32, round
-// robin; lane % 16 is the lane's query throughout (grp = lane / 16):
+// How 16 queries meet 32 tokens (lane % 16 = r is the lane's query throughout, grp = lane / 16):
 //   S^T  = K . Q^T   (A = 16 tokens x 32 dims, B = 32 dims x 16 queries): the lane gets tokens 4 grp + i of its query;
-//   O^T += V^T . P^T (A = V^T through the transposing read of the row-major tile, B = P straight from the S^T registers).
-// A lane loads 16 consecutive bytes of a K row; which dims those are only has to match between K and Q, so an e4m3 lane
-// takes dims 64 i + 16 grp .. + 15 and uses them as two operands.  K goes from memory to the operand registers; V passes
-// through the wave's own LDS tile (no barrier: nothing is shared between waves until the end).
-// The running maximum is raised only when a score exceeds it by more than 8 (powers of two), so most tiles need no
-// rescaling: p <= 2^8 fits every type used here and the reference point cancels in the end.
+//   O^T += V^T . P^T (A = V^T through the transposing read of the row-major LDS tile, B = P straight from the S^T registers),
+// so softmax statistics never cross queries and P needs no relayout.  The running maximum is raised only when a score
+// exceeds it by more than 8 (powers of two), so most tiles need no rescaling: p <= 2^8 fits every type used here and the
+// reference point cancels in the end.  P is rounded to 16 bits (2^-9 relative on average in bf16, as in the decode attention
+// over one history): the second product takes 16-bit operands, and its sums are 32-bit.
 template <typename T, bool FP8, int D> struct Shape {
   typedef std::conditional_t<FP8, __bf16, T> P;   // type of P and V: P carries the V scale, which fp16 could not hold
-  static constexpr int ES = FP8 ? 1 : 2, RB = D * ES;
-  static constexpr int KK = D / 32;                                   // products per 16 x 16 scores
-  static constexpr int KP = FP8 && D == 32 ? 1 : RB / 64;             // 16-byte pieces of a K row per lane
-  static constexpr int VP = RB / 32;                                  // 16-byte pieces of the V tile per lane
-  static constexpr int KC = D / 8;                                    // 16-byte pieces of a V row in LDS
-  static constexpr int QT = query_tile(D) / 16;
+  typedef typename HalfMfma<T>::vec8 kvec;
+  typedef typename HalfMfma<P>::vec8 pvec;
+  static constexpr int ES = FP8 ? 1 : 2, RB = D * ES;   // bytes per element and per row of the history
+  static constexpr int KK = D / 32;                     // products per 16 x 16 scores
+  static constexpr int KC = D / 8;                      // 16-byte pieces of a row of 16-bit values in LDS
+  static constexpr int ROW16 = RB / 16;                 // 16-byte pieces of a row of the history
 };
 
-template <typename T, bool FP8, bool PAGED, int D, int MT>
-__device__ __forceinline__ void attend_item(const SharedArgs& a, const i32x4 r0, const i32x4 r1, int h, bf16x8* lds_v,
-                                            float (*lds_scale)[kTile], float* lds_o, float (*lds_m)[64], float (*lds_l)[64]) {
+template <typename T, bool FP8, int D> struct QueryBlock {
   typedef Shape<T, FP8, D> S;
-  typedef typename HalfMfma<T>::vec8 kvec;
-  typedef typename HalfMfma<typename S::P>::vec8 pvec;
-  typedef typename S::P P;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, grp = lane >> 4;
-  const int row0 = r0[0], rows = r0[1], q0 = r0[2] * query_tile(D), offset = r0[3];
-  const int t0 = r1[0], t1 = r1[1], source = PAGED && !r1[3] ? row0 : r1[2], total = rows * a.G;
-  const int32_t* const row_records = a.schedule + kHeader;
-  bool bad = source < 0 || source >= a.sources;
-  const int64_t base = (PAGED || bad ? 0 : (int64_t)source * a.c0) + (int64_t)h * a.c2;
+  typename S::kvec q[S::KK];
+  f32x4 o[D / 16];
+  float m, l;
+  int limit, place;   // the query's last visible token + 1; row of the partial results, -1: nowhere
 
-  // ---- the queries
-  kvec qf[MT][S::KK];
-  int limit[MT], least = t1;
+  __device__ __forceinline__ void start(const SharedArgs& a, const i32x4 r0, int t1, int h, int q0) {
+    const int lane = threadIdx.x & 63, r = lane & 15, grp = lane >> 4;
+    const int row0 = r0[0], total = r0[1] * a.G, qi = min(q0 + r, total - 1);
+    const int b = row0 + qi / a.G, head = h * a.G + qi % a.G;
+    const T* src = (const T*)a.q + ((int64_t)b * a.QH + head) * D;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    int qi = q0 + 16 * mt + r;
-    qi = qi < total ? qi : total - 1;
-    const int b = row0 + qi / a.G;
-    const T* src = (const T*)a.q + ((int64_t)b * a.QH + h * a.G + qi % a.G) * D;
+    for (int kk = 0; kk < S::KK; ++kk) q[kk] = *reinterpret_cast<const typename S::kvec*>(src + 32 * kk + 8 * grp);
+    const i32x4 record = *reinterpret_cast<const i32x4*>(a.schedule + kHeader + kRowInts * b);
+    const int len = record[3];
+    limit = len > 0 && len < t1 ? len : t1;   // a row that sits out computes something that is never stored
+    place = q0 + r < total && len > 0 ? (record[0] + r0[3]) * a.QH + head : -1;
+    m = -kInf;
+    l = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < S::KK; ++kk) {
-      const int dim = !FP8 || D == 32 ? 32 * kk + 8 * grp : 64 * (kk >> 1) + 16 * grp + 8 * (kk & 1);
-      qf[mt][kk] = *reinterpret_cast<const kvec*>(src + dim);
-    }
-    const int len = row_records[kRowInts * b + 3];
-    limit[mt] = len > 0 && len < t1 ? len : t1;   // a row that sits out computes something that is never stored
-    least = limit[mt] < least ? limit[mt] : least;
-  }
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o, 64));
-
-  f32x4 o[MT][D / 16];
-  float m[MT], l[MT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    m[mt] = -kInf;
-    l[mt] = 0.f;
-#pragma unroll
-    for (int dd = 0; dd < D / 16; ++dd) o[mt][dd] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int dd = 0; dd < D / 16; ++dd) o[dd] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto token_offset = [&](int t) -> int64_t {   // elements, for a token of the item
-    if (PAGED) {
-      const int blk = a.page_shift >= 0 ? t >> a.page_shift : t / a.page;
-      int pool = bad ? 0 : a.table[(int64_t)source * a.max_blocks + blk];
-      if (pool < 0 || pool >= a.pools) { bad = true; pool = 0; }
-      return base + (int64_t)pool * a.c0 + (int64_t)(t - blk * a.page) * a.c1;
+  // 16 SUB tokens from T0 on; k_of(j, kk): the operand of tokens 16 j .. 16 j + 15; ksc, vsc: their scales (e4m3 only, the
+  // score scale included in the first); v: the rows of V in LDS.  More tokens at a time give the wave independent work for
+  // the latencies of the products and exponentials.
+  template <int SUB, typename F>
+  __device__ __forceinline__ void step(const SharedArgs& a, int T0, bool edge, F k_of, const float* ksc, const float* vsc, const bf16x8* v) {
+    typedef typename S::P P;
+    constexpr int N = 4 * SUB;
+    const int lane = threadIdx.x & 63, r = lane & 15, grp = lane >> 4;
+    float s[N];
+#pragma unroll
+    for (int j = 0; j < SUB; ++j) {
+      f32x4 st = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < S::KK; ++kk) st = HalfMfma<T>::run(k_of(j, kk), q[kk], st);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * j + i] = FP8 ? st[i] * ksc[4 * j + i] : st[i];
     }
-    return base + (int64_t)t * a.c1;
-  };
-  struct Raw { i32x4 k[2][S::KP], v[S::VP]; float ks, vs; };
-  auto fetch = [&](int T0, Raw& x) {
+    if (edge) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      int t = T0 + 16 * j + r;
-      t = t < t1 ? t : t1 - 1;
-      const uint8_t* row = (const uint8_t*)a.kc + token_offset(t) * S::ES;
-      if constexpr (FP8 && D == 32) {
-        const i32x2 half = *reinterpret_cast<const i32x2*>(row + 8 * grp);
-        x.k[j][0] = i32x4{half[0], half[1], 0, 0};
-      } else {
-#pragma unroll
-        for (int i = 0; i < S::KP; ++i) x.k[j][i] = *reinterpret_cast<const i32x4*>(row + 64 * i + 16 * grp);
-      }
+      for (int i = 0; i < N; ++i) s[i] = T0 + 16 * (i >> 2) + 4 * grp + (i & 3) < limit ? s[i] : -kInf;
     }
+    float mx = s[0];
 #pragma unroll
-    for (int u = 0; u < S::VP; ++u) {
-      constexpr int per_row = S::RB / 16;
-      const int piece = lane + 64 * u;
-      int t = T0 + piece / per_row;
-      t = t < t1 ? t : t1 - 1;
-      x.v[u] = *reinterpret_cast<const i32x4*>((const uint8_t*)a.vc + token_offset(t) * S::ES + 16 * (piece % per_row));
+    for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
+    if constexpr (!FP8) mx *= a.scale_log2e;   // the scale is positive: scores stay unscaled until the exponential
+    if (__any(mx > m + 8.0f)) {
+      mx = max_lane_xor32(max_lane_xor16(mx));
+      const float mnew = fmaxf(m, mx);
+      const float alpha = mnew == -kInf ? 1.f : __builtin_amdgcn_exp2f(m - mnew);
+      m = mnew;
+      l *= alpha;
+#pragma unroll
+      for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[dd][i] *= alpha;
     }
-    if constexpr (FP8) {
-      int t = T0 + (lane & 31);
-      t = t < t1 ? t : t1 - 1;
-      const int64_t at = token_offset(t) / D;
-      x.ks = a.ks[at];
-      x.vs = a.vs[at];
+    const float ref = m == -kInf ? 0.f : m;   // nothing seen yet: every score here is masked, p = 0
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    typename S::pvec pf[SUB / 2];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float p = __builtin_amdgcn_exp2f(FP8 ? s[i] - ref : fmaf(s[i], a.scale_log2e, -ref));
+      sum[i & 3] += p;
+      pf[i >> 3][i & 7] = (P)(FP8 ? p * vsc[i] : p);
     }
-  };
-
-  const int first = t0 + wave * kTile;
-  Raw raw;
-  if (first < t1 && !(bad && !PAGED)) {
-    fetch(first, raw);
-    for (int T0 = first; T0 < t1; T0 += kGrain) {
-      const bool edge = T0 + kTile > least;
-      // ---- this tile: V to LDS, K to operands
-      kvec kf[2][S::KK];
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    // tokens 4 grp + i and 16 + 4 grp + i (of each 32) of dim 16 dd + r: the order P holds them in
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+    for (int dd = 0; dd < D / 16; ++dd) {
 #pragma unroll
-        for (int kk = 0; kk < S::KK; ++kk) {
-          if constexpr (!FP8) kf[j][kk] = __builtin_bit_cast(kvec, raw.k[j][kk]);
-          else if constexpr (D == 32) kf[j][kk] = widen8<T>(raw.k[j][0][0], raw.k[j][0][1]);
-          else kf[j][kk] = widen8<T>(raw.k[j][kk >> 1][2 * (kk & 1)], raw.k[j][kk >> 1][2 * (kk & 1) + 1]);
-        }
-#pragma unroll
-      for (int u = 0; u < S::VP; ++u) {
-        constexpr int per_row = S::RB / 16;
-        const int piece = lane + 64 * u, tok = piece / per_row, c = piece % per_row;
-        i32x4 w = raw.v[u];
-        if (T0 + tok >= t1) w = i32x4{0, 0, 0, 0};   // 0 * whatever the last row holds
-        if constexpr (FP8) {
-          const bf16x8 lo = widen8<__bf16>(w[0], w[1]), hi = widen8<__bf16>(w[2], w[3]);
-          lds_v[tok * S::KC + ((2 * c) ^ (tok & (S::KC - 1)))] = lo;
-          lds_v[tok * S::KC + ((2 * c + 1) ^ (tok & (S::KC - 1)))] = hi;
-        } else {
-          lds_v[tok * S::KC + (c ^ (tok & (S::KC - 1)))] = __builtin_bit_cast(bf16x8, w);
-        }
-      }
-      float ksc[8], vsc[8];
-      if constexpr (FP8) {
-        if (lane < kTile) { lds_scale[0][lane] = raw.ks * a.scale_log2e; lds_scale[1][lane] = raw.vs; }
+      for (int half = 0; half < SUB / 2; ++half) {
+        s16x4 piece[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const f32x4 k4 = *reinterpret_cast<const f32x4*>(&lds_scale[0][16 * j + 4 * grp]);
-          const f32x4 v4 = *reinterpret_cast<const f32x4*>(&lds_scale[1][16 * j + 4 * grp]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { ksc[4 * j + i] = k4[i]; vsc[4 * j + i] = v4[i]; }
-        }
-      }
-      if (T0 + kGrain < t1) fetch(T0 + kGrain, raw);
-
-      // ---- scores and probabilities of every query block
-      pvec pf[MT];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        float s[8];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          f32x4 st = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int kk = 0; kk < S::KK; ++kk) st = HalfMfma<T>::run(kf[j][kk], qf[mt][kk], st);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[4 * j + i] = st[i] * (FP8 ? ksc[4 * j + i] : a.scale_log2e);
-        }
-        if (edge) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[4 * j + i] = T0 + 16 * j + 4 * grp + i < limit[mt] ? s[4 * j + i] : -kInf;
-        }
-        float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-        if (__any(mx > m[mt] + 8.0f)) {
-          mx = max_lane_xor32(max_lane_xor16(mx));
-          const float mnew = fmaxf(m[mt], mx);
-          const float alpha = mnew == -kInf ? 1.f : __builtin_amdgcn_exp2f(m[mt] - mnew);
-          m[mt] = mnew;
-          l[mt] *= alpha;
-#pragma unroll
-          for (int dd = 0; dd < D / 16; ++dd)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[mt][dd][i] *= alpha;
-        }
-        const float ref = m[mt] == -kInf ? 0.f : m[mt];   // nothing seen yet: every score here is masked, p = 0
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p = __builtin_amdgcn_exp2f(s[i] - ref);
-          sum += p;
-          pf[mt][i] = (P)(FP8 ? p * vsc[i] : p);
-        }
-        l[mt] += sum;
-      }
-      // ---- O^T += V^T . P^T: tokens 4 grp + i and 16 + 4 grp + i of dim 16 dd + r, the order P holds them in
-#pragma unroll
-      for (int dd = 0; dd < D / 16; ++dd) {
-        s16x4 half[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int tok = 16 * j + 4 * grp + (r >> 2), c = 2 * dd + ((r & 3) >> 1);
-          const char* piece = reinterpret_cast<const char*>(&lds_v[tok * S::KC + (c ^ (tok & (S::KC - 1)))]) + 8 * (r & 1);
-          half[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)piece);
+          const int tok = 32 * half + 16 * j + 4 * grp + (r >> 2), c = 2 * dd + ((r & 3) >> 1);
+          const char* at = reinterpret_cast<const char*>(v + tok * S::KC + (c ^ (tok & (S::KC - 1)))) + 8 * (r & 1);
+          piece[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
         }
         typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const s16x8 both = {half[0][0], half[0][1], half[0][2], half[0][3], half[1][0], half[1][1], half[1][2], half[1][3]};
-        const pvec vf = __builtin_bit_cast(pvec, both);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) o[mt][dd] = HalfMfma<P>::run(vf, pf[mt], o[mt][dd]);
+        const s16x8 both = {piece[0][0], piece[0][1], piece[0][2], piece[0][3], piece[1][0], piece[1][1], piece[1][2], piece[1][3]};
+        o[dd] = HalfMfma<P>::run(__builtin_bit_cast(typename S::pvec, both), pf[half], o[dd]);
       }
     }
   }
 
-  // ---- the four waves' partial results meet: statistics first, then one query block of O at a time
-  bad = __any(bad);
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    l[mt] = add_lane_xor32(add_lane_xor16(l[mt]));
-    if (bad) l[mt] = __builtin_nanf("");   // a slot or page outside the cache
-    if (grp == 0) { lds_m[wave][16 * mt + r] = m[mt]; lds_l[wave][16 * mt + r] = l[mt]; }
+  __device__ __forceinline__ void finish(bool bad) {   // row sums; a slot or page outside the cache makes them NaN
+    l = add_lane_xor32(add_lane_xor16(l));
+    if (bad) l = __builtin_nanf("");
   }
-  __syncthreads();
+  __device__ __forceinline__ void store(const SharedArgs& a) const {
+    const int grp = (threadIdx.x & 63) >> 4;
+    if (place < 0) return;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int q = 16 * mt + r;
-    const float mm = fmaxf(fmaxf(lds_m[0][q], lds_m[1][q]), fmaxf(lds_m[2][q], lds_m[3][q]));
-    const float f = mm == -kInf ? 0.f : __builtin_amdgcn_exp2f(m[mt] - mm);
-#pragma unroll
-    for (int dd = 0; dd < D / 16; ++dd)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) lds_o[(wave * 16 + r) * (D + 4) + 16 * dd + 4 * grp + i] = o[mt][dd][i] * f;
-    __syncthreads();
-    for (int at = threadIdx.x; at < 16 * (D / 4); at += 256) {
-      const int query = at / (D / 4), d = 4 * (at % (D / 4)), qi = q0 + 16 * mt + query;
-      if (qi < total) {
-        const int b = row0 + qi / a.G;
-        const int32_t* row = row_records + kRowInts * b;
-        if (row[3] > 0) {
-          f32x4 sum = *reinterpret_cast<const f32x4*>(&lds_o[query * (D + 4) + d]);
-#pragma unroll
-          for (int w = 1; w < 4; ++w) sum += *reinterpret_cast<const f32x4*>(&lds_o[(w * 16 + query) * (D + 4) + d]);
-          const int64_t at_row = (int64_t)(row[0] + offset) * a.QH + h * a.G + qi % a.G;
-          *reinterpret_cast<f32x4*>(a.acc + at_row * D + d) = sum;
-          if (d == 0) {
-            const int qq = 16 * mt + query;
-            const float top = fmaxf(fmaxf(lds_m[0][qq], lds_m[1][qq]), fmaxf(lds_m[2][qq], lds_m[3][qq]));
-            float lt = 0.f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) lt += lds_l[w][qq] * (top == -kInf ? 1.f : __builtin_amdgcn_exp2f(lds_m[w][qq] - top));
-            a.m[at_row] = top;
-            a.l[at_row] = lt;
-          }
-        }
-      }
+    for (int dd = 0; dd < D / 16; ++dd) *reinterpret_cast<f32x4*>(a.acc + (int64_t)place * D + 16 * dd + 4 * grp) = o[dd];
+    if (grp == 0) { a.m[place] = m; a.l[place] = l; }
+  }
+};
+
+// Where the tokens of an item are.  Dense: base + t * c1; paged: through the table row.
+template <bool PAGED> struct History {
+  const SharedArgs& a;
+  int64_t base;
+  int table_row;
+  bool bad;   // a slot or page outside the cache: nothing there is read
+  __device__ __forceinline__ History(const SharedArgs& args, int source, int h) : a(args), table_row(source) {
+    bad = source < 0 || source >= a.sources;
+    base = (PAGED || bad ? 0 : (int64_t)source * a.c0) + (int64_t)h * a.c2;
+  }
+  __device__ __forceinline__ int64_t offset(int t) {   // in elements
+    if constexpr (PAGED) {
+      const int block = a.page_shift >= 0 ? t >> a.page_shift : t / a.page;
+      int pool = bad ? 0 : a.table[(int64_t)table_row * a.max_blocks + block];
+      if (pool < 0 || pool >= a.pools) { bad = true; pool = 0; }
+      return base + (int64_t)pool * a.c0 + (int64_t)(t - block * a.page) * a.c1;
     }
-    __syncthreads();
+    return base + (int64_t)t * a.c1;
+  }
+};
+
+// 16 bytes of a V row (or of a K row) to LDS as 16-bit values: piece c of row `tok`, swizzled by the row so that the stores
+// and both kinds of read spread over the banks.
+template <typename T, bool FP8, int D> __device__ __forceinline__ void stage(bf16x8* rows, int tok, int c, const i32x4 w) {
+  constexpr int KC = Shape<T, FP8, D>::KC;
+  if constexpr (FP8) {
+    rows[tok * KC + ((2 * c) ^ (tok & (KC - 1)))] = __builtin_bit_cast(bf16x8, widen8<T>(w[0], w[1]));
+    rows[tok * KC + ((2 * c + 1) ^ (tok & (KC - 1)))] = __builtin_bit_cast(bf16x8, widen8<T>(w[2], w[3]));
+  } else {
+    rows[tok * KC + (c ^ (tok & (KC - 1)))] = __builtin_bit_cast(bf16x8, w);
   }
 }
 
-template <typename T, bool FP8, bool PAGED, int D>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) shared_attention_kernel(SharedArgs a) {
+// The way of K and V rows from memory to LDS: THREADS threads bring TOKENS tokens, consecutive threads consecutive 16-byte
+// pieces, so that every load instruction asks for whole cache lines.
+template <typename T, bool FP8, bool PAGED, int D, int THREADS, int TOKENS, bool STREAM> struct Rows {
   typedef Shape<T, FP8, D> S;
-  __shared__ bf16x8 lds_v[4][kTile * S::KC];
-  __shared__ __attribute__((aligned(16))) float lds_scale[4][2][kTile];
-  __shared__ __attribute__((aligned(16))) float lds_o[4 * 16 * (D + 4)];
-  __shared__ float lds_m[4][64], lds_l[4][64];
+  static constexpr int N = TOKENS * S::ROW16 / THREADS;          // pieces per thread, of K and of V
+  static constexpr int NS = !FP8 ? 0 : THREADS >= 2 * TOKENS ? 1 : 2;   // scales per thread (K and V, or one of the two)
+  static_assert(N >= 1 && (!FP8 || THREADS >= TOKENS), "a thread has a piece, and a token a thread");
+  struct Raw { i32x4 k[N], v[N]; float s[NS > 0 ? NS : 1]; };
+  const SharedArgs& a;
+  History<PAGED>& history;
+  const int t1, thread, row_bytes;
+  uint32_t whole[N];
+  __device__ __forceinline__ Rows(const SharedArgs& args, History<PAGED>& h, int end, int id)
+      : a(args), history(h), t1(end), thread(id), row_bytes((int)args.c1 * S::ES) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) whole[i] = row_of(i) * row_bytes + 16 * piece_of(i);
+  }
+  __device__ __forceinline__ int row_of(int i) const { return (thread + THREADS * i) / S::ROW16; }
+  __device__ __forceinline__ int piece_of(int i) const { return (thread + THREADS * i) % S::ROW16; }
+  // A history that is read once per step and by one workgroup leaves nothing in the caches that anybody wants: the
+  // non-temporal hint (streaming reads run at 6.9 TB/s with it and 6.1 without).
+  template <typename V> static __device__ __forceinline__ V load(const V* p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(p);
+    else return *p;
+  }
+  // tokens from T0 on, cut to the item's; past its end, its last token for every thread
+  __device__ __forceinline__ void fetch(int T0, Raw& x) {
+    T0 = T0 < t1 ? T0 : t1 - 1;
+    const int last = t1 - 1 - T0;
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int64_t at = history.offset(T0 + min(row_of(i), last)) * S::ES + 16 * piece_of(i);
+        x.k[i] = load(reinterpret_cast<const i32x4*>((const uint8_t*)a.kc + at));
+        x.v[i] = load(reinterpret_cast<const i32x4*>((const uint8_t*)a.vc + at));
+      }
+      if constexpr (FP8) load_scales(history.offset(T0 + min(thread % TOKENS, last)) / D, x);
+    } else {
+      const int64_t start = history.offset(T0);
+      const uint8_t* krows = (const uint8_t*)a.kc + start * S::ES;
+      const uint8_t* vrows = (const uint8_t*)a.vc + start * S::ES;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        uint32_t at = whole[i];
+        if (last < TOKENS - 1) at = min(row_of(i), last) * row_bytes + 16 * piece_of(i);
+        x.k[i] = load(reinterpret_cast<const i32x4*>(krows + at));
+        x.v[i] = load(reinterpret_cast<const i32x4*>(vrows + at));
+      }
+      if constexpr (FP8) load_scales(start / D + (uint32_t)min(thread % TOKENS, last) * (uint32_t)(row_bytes / D), x);
+    }
+  }
+  __device__ __forceinline__ void load_scales(int64_t at, Raw& x) const {
+    if constexpr (NS == 2) { x.s[0] = load(a.ks + at); x.s[1] = load(a.vs + at); }
+    if constexpr (NS == 1) x.s[0] = load((thread < TOKENS ? a.ks : a.vs) + at);
+  }
+  // pieces [first, first + COUNT) of the thread, the first of them belonging to token `base` of the LDS tile's 0
+  template <int FIRST, int COUNT> __device__ __forceinline__ void stage_k(const Raw& x, bf16x8* rows) const {
+#pragma unroll
+    for (int i = FIRST; i < FIRST + COUNT; ++i) stage<T, FP8, D>(rows, row_of(i) - FIRST * THREADS / S::ROW16, piece_of(i), x.k[i]);
+  }
+  template <int FIRST, int COUNT> __device__ __forceinline__ void stage_v(const Raw& x, int T0, bf16x8* rows) const {
+#pragma unroll
+    for (int i = FIRST; i < FIRST + COUNT; ++i) {
+      i32x4 w = x.v[i];
+      if (T0 + row_of(i) >= t1) w = i32x4{0, 0, 0, 0};   // 0 * whatever the last row holds
+      stage<typename S::P, FP8, D>(rows, row_of(i) - FIRST * THREADS / S::ROW16, piece_of(i), w);
+    }
+  }
+  __device__ __forceinline__ void stage_scales(const Raw& x, float* k_scale, float* v_scale) const {
+    if constexpr (NS == 2) {
+      if (thread < TOKENS) { k_scale[thread] = x.s[0] * a.scale_log2e; v_scale[thread] = x.s[1]; }
+    }
+    if constexpr (NS == 1) {
+      if (thread < TOKENS) k_scale[thread] = x.s[0] * a.scale_log2e;
+      else if (thread < 2 * TOKENS) v_scale[thread - TOKENS] = x.s[0];
+    }
+  }
+};
+
+// The scales of the lane's 4 SUB tokens of a step.
+template <int SUB> __device__ __forceinline__ void read_scales(const float* k_scale, const float* v_scale, int grp, float* ksc, float* vsc) {
+#pragma unroll
+  for (int j = 0; j < SUB; ++j) {
+    const f32x4 k4 = *reinterpret_cast<const f32x4*>(k_scale + 16 * j + 4 * grp);
+    const f32x4 v4 = *reinterpret_cast<const f32x4*>(v_scale + 16 * j + 4 * grp);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { ksc[4 * j + i] = k4[i]; vsc[4 * j + i] = v4[i]; }
+  }
+}
+// A wave's smallest limit: from there on its scores need the mask.
+__device__ __forceinline__ int wave_least(int limit) {
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) limit = min(limit, __shfl_xor(limit, o, 64));
+  return __builtin_amdgcn_readfirstlane(limit);
+}
+
+// An item of one block of queries against tokens [t0, t1) of one KV head.  A wave works by itself on tiles of 4 KiB of K and
+// of V (at least 32 tokens): the next one is on its way to registers while the rows of the current one pass through the
+// wave's own LDS, 32 tokens at a time.  The four waves of a workgroup share a long item, taking its tiles round robin (the
+// four then read 16 KiB in a row), and their results meet at its end; a short item is one wave's.
+template <typename T, bool FP8, bool PAGED, int D, bool LONG>
+__device__ __forceinline__ void block_item(const SharedArgs& a, const i32x4 r0, const i32x4 r1, int h, bf16x8* lds, float* lds_scale) {
+  typedef Shape<T, FP8, D> S;
+  constexpr int TOKENS = 4096 / S::RB > 64 ? 64 : 4096 / S::RB < 32 ? 32 : 4096 / S::RB;
+  constexpr int PARTS = TOKENS / kStep, STRIDE = LONG ? 4 * TOKENS : TOKENS;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, grp = lane >> 4;
+  bf16x8* const lds_k = lds + wave * 2 * kStep * S::KC;
+  bf16x8* const lds_v = lds_k + kStep * S::KC;
+  float* const k_scale = lds_scale + wave * 128;
+  float* const v_scale = k_scale + 64;
+  const int t0 = r1[0] + (LONG ? wave * TOKENS : 0), t1 = r1[1];
+  History<PAGED> history(a, PAGED && !r1[3] ? r0[0] : r1[2], h);
+  typedef Rows<T, FP8, PAGED, D, 64, TOKENS, true> Tile;
+  Tile tile(a, history, t1, lane);
+  typename Tile::Raw raw;
+  const bool work = t0 < t1 && (PAGED || !history.bad);   // the same for the whole wave
+  if (work) tile.fetch(t0, raw);
+  QueryBlock<T, FP8, D> block;
+  block.start(a, r0, t1, h, r0[2] * kQueryBlock);
+  const int least = wave_least(block.limit);
+  if (work) {
+    for (int T0 = t0; T0 < t1; T0 += STRIDE) {
+      typename Tile::Raw now = raw;
+      auto part = [&](auto index) __attribute__((always_inline)) {
+        constexpr int PART = decltype(index)::value, COUNT = Tile::N / PARTS;
+        const int from = T0 + kStep * PART;
+        wave_sync();
+        tile.template stage_k<PART * COUNT, COUNT>(now, lds_k);
+        tile.template stage_v<PART * COUNT, COUNT>(now, T0, lds_v);
+        if constexpr (FP8 && PART == 0) tile.stage_scales(now, k_scale, v_scale);
+        wave_sync();
+        if constexpr (PART == PARTS - 1) tile.fetch(T0 + STRIDE, raw);
+        float ksc[8], vsc[8];
+        if constexpr (FP8) read_scales<2>(k_scale + kStep * PART, v_scale + kStep * PART, grp, ksc, vsc);
+        if (PART == 0 || from < t1)
+          block.template step<2>(a, from, from + kStep > least, [&](int j, int kk) {
+            const int tok = 16 * j + r;
+            return __builtin_bit_cast(typename S::kvec, lds_k[tok * S::KC + ((4 * kk + grp) ^ (tok & (S::KC - 1)))]);
+          }, ksc, vsc, lds_v);
+      };
+      part(std::integral_constant<int, 0>{});
+      if constexpr (PARTS == 2) part(std::integral_constant<int, 1>{});
+    }
+  }
+  block.finish(__any(history.bad));
+  if constexpr (LONG) {   // the four results meet: each wave's O, m and l, lane by lane
+    float* const share = reinterpret_cast<float*>(lds);
+    constexpr int AREA = 64 * (D / 4 + 2);
+    __syncthreads();
+    if (wave > 0) {
+      float* const to = share + (wave - 1) * AREA;
+#pragma unroll
+      for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[(4 * dd + i) * 64 + lane] = block.o[dd][i];
+      to[D / 4 * 64 + lane] = block.m;
+      to[(D / 4 + 1) * 64 + lane] = block.l;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      float mw[4], mm = block.m;
+      mw[0] = block.m;
+#pragma unroll
+      for (int w = 1; w < 4; ++w) { mw[w] = share[(w - 1) * AREA + D / 4 * 64 + lane]; mm = fmaxf(mm, mw[w]); }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mw[w] = mm == -kInf ? 1.f : __builtin_amdgcn_exp2f(mw[w] - mm);
+      block.m = mm;
+      block.l *= mw[0];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) block.l = fmaf(share[(w - 1) * AREA + (D / 4 + 1) * 64 + lane], mw[w], block.l);
+#pragma unroll
+      for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = block.o[dd][i] * mw[0];
+#pragma unroll
+          for (int w = 1; w < 4; ++w) v = fmaf(share[(w - 1) * AREA + (4 * dd + i) * 64 + lane], mw[w], v);
+          block.o[dd][i] = v;
+        }
+      block.store(a);
+    }
+    __syncthreads();   // the next item's tiles go where the results met
+  } else {
+    block.store(a);
+  }
+}
+
+// A shared item: up to 64 queries of a group against tokens [t0, t1) of one KV head, 128 tokens at a time.  All four waves
+// stage the tile (the next ones are on their way to registers meanwhile); then wave w takes query block w, or, with at most
+// two blocks, block w % 2 and half w / 2 of the tile's tokens, whose two results meet at the end.
+template <typename T, bool FP8, bool PAGED, int D>
+__device__ __forceinline__ void shared_item(const SharedArgs& a, const i32x4 r0, const i32x4 r1, int h, bf16x8* lds, float* lds_scale) {
+  typedef Shape<T, FP8, D> S;
+  bf16x8* const lds_k = lds;
+  bf16x8* const lds_v = lds + kShareTile * S::KC;
+  float* const k_scale = lds_scale;
+  float* const v_scale = lds_scale + kShareTile;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, grp = lane >> 4;
+  const int t0 = r1[0], t1 = r1[1];
+  const int q0 = r0[2] * kQueryTile, blocks = (min(r0[1] * a.G - q0, kQueryTile) + 15) / 16;
+  const bool halves = blocks <= 2;
+  const int mine = halves ? wave & 1 : wave;
+  const bool busy = mine < blocks;
+  History<PAGED> history(a, r1[2], h);
+  typedef Rows<T, FP8, PAGED, D, 256, kShareTile, false> Tile;
+  Tile tile(a, history, t1, threadIdx.x);
+  typename Tile::Raw raw;
+  const bool readable = PAGED || !history.bad;
+  if (readable) tile.fetch(t0, raw);
+  QueryBlock<T, FP8, D> block;
+  block.start(a, r0, t1, h, q0 + 16 * mine);
+  if (!busy) block.place = -1;
+  const int least = wave_least(block.limit);
+  constexpr int SUB = D <= 64 ? 4 : 2, STEP = 16 * SUB, STEPS = kShareTile / STEP;
+  const int first = halves ? STEPS / 2 * (wave >> 1) : 0, count = halves ? STEPS / 2 : STEPS;   // the wave's steps of a tile
+  if (readable) {
+    for (int T0 = t0; T0 < t1; T0 += kShareTile) {
+      __syncthreads();
+      tile.template stage_k<0, Tile::N>(raw, lds_k);
+      tile.template stage_v<0, Tile::N>(raw, T0, lds_v);
+      if constexpr (FP8) tile.stage_scales(raw, k_scale, v_scale);
+      __syncthreads();
+      tile.fetch(T0 + kShareTile, raw);
+      if (busy) {
+        for (int part = first; part < first + count; ++part) {
+          const int row = STEP * part, from = T0 + row;
+          if (from >= t1) break;
+          float ksc[4 * SUB], vsc[4 * SUB];
+          if constexpr (FP8) read_scales<SUB>(k_scale + row, v_scale + row, grp, ksc, vsc);
+          block.template step<SUB>(a, from, from + STEP > least, [&](int j, int kk) {
+            const int tok = row + 16 * j + r;
+            return __builtin_bit_cast(typename S::kvec, lds_k[tok * S::KC + ((4 * kk + grp) ^ (tok & (S::KC - 1)))]);
+          }, ksc, vsc, lds_v + row * S::KC);
+        }
+      }
+    }
+  }
+  block.finish(__syncthreads_or(history.bad));   // also: the last tile has been read by all waves
+  if (halves) {   // waves 2 and 3 hand their results to waves 0 and 1
+    float* const other = reinterpret_cast<float*>(lds) + (wave & 1) * 64 * (D / 4 + 2);   // lane by lane: O, then m and l
+    if (wave >= 2) {
+#pragma unroll
+      for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) other[(4 * dd + i) * 64 + lane] = block.o[dd][i];
+      other[D / 4 * 64 + lane] = block.m;
+      other[(D / 4 + 1) * 64 + lane] = block.l;
+    }
+    __syncthreads();
+    if (wave < 2) {
+      const float om = other[D / 4 * 64 + lane], mm = fmaxf(block.m, om);
+      const float fa = mm == -kInf ? 1.f : __builtin_amdgcn_exp2f(block.m - mm), fb = mm == -kInf ? 1.f : __builtin_amdgcn_exp2f(om - mm);
+      block.l = block.l * fa + other[(D / 4 + 1) * 64 + lane] * fb;
+      block.m = mm;
+#pragma unroll
+      for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) block.o[dd][i] = fmaf(other[(4 * dd + i) * 64 + lane], fb, block.o[dd][i] * fa);
+    } else {
+      block.place = -1;
+    }
+  }
+  block.store(a);
+  __syncthreads();   // the next item's tiles go where the halves met
+}
+
+template <typename T, bool FP8, bool PAGED, int D>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3 : 2))) shared_attention_kernel(SharedArgs a) {
+  typedef Shape<T, FP8, D> S;
+  __shared__ bf16x8 lds[2 * kShareTile * S::KC];   // K and V: 32 tokens for each wave, or 128 for the workgroup
+  __shared__ __attribute__((aligned(16))) float lds_scale[4 * 128];
+  static_assert(3 * 64 * (D / 4 + 2) * 4 <= (int)sizeof(lds), "the waves' results fit the tile memory");
   if (!list_fits(a, D)) return;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int32_t* const records = a.schedule + kHeader + kRowInts * a.B;
-  const int items = a.schedule[kHRecords] * a.KH;
-  for (int idx = blockIdx.x; idx < items; idx += gridDim.x) {
-    const i32x4* rec = reinterpret_cast<const i32x4*>(records + (int64_t)kRecordInts * (idx / a.KH));
-    const i32x4 r0 = rec[0], r1 = rec[1];
-    const int h = idx % a.KH;
-    const int queries = min(r0[1] * a.G - r0[2] * query_tile(D), query_tile(D));
-    if (queries <= 16) attend_item<T, FP8, PAGED, D, 1>(a, r0, r1, h, lds_v[wave], lds_scale[wave], lds_o, lds_m, lds_l);
-    else if (queries <= 32 || S::QT == 2) attend_item<T, FP8, PAGED, D, 2>(a, r0, r1, h, lds_v[wave], lds_scale[wave], lds_o, lds_m, lds_l);
-    else attend_item<T, FP8, PAGED, D, S::QT>(a, r0, r1, h, lds_v[wave], lds_scale[wave], lds_o, lds_m, lds_l);
+  const int shared_records = a.schedule[kHShared], long_records = a.schedule[kHLong], short_records = a.schedule[kHShort];
+  auto record = [&](int at, i32x4& r0, i32x4& r1) {   // the same in every lane
+    const i32x4* rec = reinterpret_cast<const i32x4*>(records + (int64_t)kRecordInts * at);
+    auto scalar = [](const i32x4 v) {
+      return i32x4{__builtin_amdgcn_readfirstlane(v[0]), __builtin_amdgcn_readfirstlane(v[1]), __builtin_amdgcn_readfirstlane(v[2]),
+                   __builtin_amdgcn_readfirstlane(v[3])};
+    };
+    r0 = scalar(rec[0]);
+    r1 = scalar(rec[1]);
+  };
+  i32x4 r0, r1;
+  // The first 2 * shared_blocks workgroups take shared and other items in turn, the rest other items: what runs at the same
+  // time on a CU is some of each (shared parts are bound by arithmetic, the others by memory).  A turn is one workgroup for
+  // every CU: consecutive workgroups go to the XCDs, their shader engines and CUs in turn, so that a shorter period would
+  // give all shared items to some of them (turns of 8 workgroups: shared parts alone took 99 us, now XXX).  The grid fills the
+  // chip about once and strides over the items: a workgroup without work costs its slot a microsecond or two.
+  int block = blockIdx.x;
+  if (block < 2 * a.shared_blocks && block % (2 * kTurn) < kTurn) {
+    for (int idx = block / (2 * kTurn) * kTurn + block % kTurn; idx < shared_records * a.KH; idx += a.shared_blocks) {
+      record(idx / a.KH, r0, r1);
+      shared_item<T, FP8, PAGED, D>(a, r0, r1, idx % a.KH, lds, lds_scale);
+    }
+    return;
+  }
+  block = block < 2 * a.shared_blocks ? block / (2 * kTurn) * kTurn + block % kTurn : block - a.shared_blocks;
+  for (int idx = block; idx < long_records * a.KH; idx += a.other_blocks) {
+    record(shared_records + idx / a.KH, r0, r1);
+    block_item<T, FP8, PAGED, D, true>(a, r0, r1, idx % a.KH, lds, lds_scale);
+  }
+  for (int idx = block * 4 + wave; idx < short_records * a.KH; idx += 4 * a.other_blocks) {
+    record(shared_records + long_records + idx / a.KH, r0, r1);
+    block_item<T, FP8, PAGED, D, false>(a, r0, r1, idx % a.KH, lds, lds_scale);
   }
 }
 
@@ -578,12 +806,12 @@ extern "C" {
 
 int64_t lfm2_shared_schedule_size(int64_t B, int64_t capacity, int QH, int KH, int D) {
   if (check_batch("shared_schedule_size", B, QH, KH, D, capacity)) return 0;
-  return schedule_ints(B, capacity, QH / KH, D);
+  return schedule_ints(B, capacity, QH / KH);
 }
 
 int64_t lfm2_shared_attention_workspace(int64_t B, int64_t capacity, int QH, int KH, int D) {
   if (check_batch("shared_attention_workspace", B, QH, KH, D, capacity)) return 0;
-  return slot_bounds(B, capacity, QH / KH, D).slots * QH * (D + 2);
+  return slot_bounds(B, capacity, QH / KH).slots * QH * (D + 2);
 }
 
 int lfm2_shared_schedule(int32_t* schedule, const int32_t* positions, const uint8_t* active, const int32_t* slot_ids,
@@ -614,7 +842,7 @@ int lfm2_shared_attention(void* out, const void* q, const void* k_cache, const v
   SharedArgs a;
   a.out = out; a.q = q; a.kc = k_cache; a.vc = v_cache; a.ks = k_scales; a.vs = v_scales;
   a.schedule = schedule; a.table = block_table;
-  const int64_t slots = slot_bounds(B, capacity, QH / KH, D).slots;
+  const int64_t slots = slot_bounds(B, capacity, QH / KH).slots;
   a.acc = workspace;
   a.m = workspace + slots * QH * D;
   a.l = a.m + slots * QH;
@@ -624,8 +852,11 @@ int lfm2_shared_attention(void* out, const void* q, const void* k_cache, const v
   a.B = (int)B; a.QH = QH; a.KH = KH; a.G = QH / KH; a.capacity = (int)capacity;
   a.scale_log2e = scale * LFM2_LOG2E;
   hipStream_t s = (hipStream_t)stream;
-  const int64_t bound = slot_bounds(B, capacity, a.G, D).records * KH;
-  const dim3 grid((unsigned)(bound < 1024 ? bound : 1024)), join((unsigned)B, (unsigned)((QH + 3) / 4));
+  // workgroups: as many as there can be items of either kind, up to a number that fills the chip and then strides
+  const int64_t most = slot_bounds(B, capacity, a.G).records * KH;
+  a.shared_blocks = most < kTurn ? kTurn : kSharedBlocks;
+  a.other_blocks = most < kTurn ? kTurn : kOtherBlocks;
+  const dim3 grid((unsigned)(a.shared_blocks + a.other_blocks)), join((unsigned)B, (unsigned)((QH + 3) / 4));
 #define SHARED_(T, FP8, PAGED, D_) hipLaunchKernelGGL((shared_attention_kernel<T, FP8, PAGED, D_>), grid, dim3(256), 0, s, a)
 #define SHARED_D_(T, D_)                                                                                              \
   do {                                                                                                                \
