@@ -289,16 +289,31 @@ __device__ __forceinline__ bool list_fits(const SharedArgs& a, int D) {
 //   O^T += V^T . P^T (A = V^T through the transposing read of the row-major LDS tile, B = P straight from the S^T registers),
 // so softmax statistics never cross queries and P needs no relayout.  The running maximum is raised only when a score
 // exceeds it by more than 8 (powers of two), so most tiles need no rescaling: p <= 2^8 fits every type used here and the
-// reference point cancels in the end.  P is rounded to 16 bits (2^-9 relative on average in bf16, as in the decode attention
-// over one history): the second product takes 16-bit operands, and its sums are 32-bit.
+// reference point cancels in the end.
+// The second product takes 16-bit operands.  A 16-bit history's P goes in as two of them, the rounded value and the rounded
+// rest (2^-16 relative in bf16: one rounding alone would be as large as the output's own).  An e4m3 history's goes in as one
+// fp16 value (2^-12), with the scale of its V row: the weight is w = 2^{s + log2 vs - m}, m a running maximum of s + log2 vs,
+// so it stays in fp16's range whatever the scales are, and the softmax sum takes w / vs.
 template <typename T, bool FP8, int D> struct Shape {
-  typedef std::conditional_t<FP8, __bf16, T> P;   // type of P and V: P carries the V scale, which fp16 could not hold
+  typedef std::conditional_t<FP8, _Float16, T> P;   // type of P and V: fp16 holds e4m3 exactly, and three more bits of P than bf16
   typedef typename HalfMfma<T>::vec8 kvec;
   typedef typename HalfMfma<P>::vec8 pvec;
   static constexpr int ES = FP8 ? 1 : 2, RB = D * ES;   // bytes per element and per row of the history
   static constexpr int KK = D / 32;                     // products per 16 x 16 scores
   static constexpr int KC = D / 8;                      // 16-byte pieces of a row of 16-bit values in LDS
   static constexpr int ROW16 = RB / 16;                 // 16-byte pieces of a row of the history
+};
+
+// Scales of a tile's tokens in LDS: of K with the score scale and log2 e, log2 of V's and its inverse.
+struct Scales {
+  float *k, *log_v, *inverse_v;
+  __device__ __forceinline__ Scales operator+(int t) const { return Scales{k + t, log_v + t, inverse_v + t}; }
+  __device__ __forceinline__ void set_v(int t, float vs) const {
+    // a scale of 0 (its row is all zeros) takes part in the softmax sum and adds nothing: 2^-80 does the same
+    vs = vs < 8.2718061e-25f ? 8.2718061e-25f : vs;
+    log_v[t] = __builtin_amdgcn_logf(vs);
+    inverse_v[t] = __builtin_amdgcn_rcpf(vs);
+  }
 };
 
 template <typename T, bool FP8, int D> struct QueryBlock {
@@ -325,11 +340,10 @@ template <typename T, bool FP8, int D> struct QueryBlock {
     for (int dd = 0; dd < D / 16; ++dd) o[dd] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // 16 SUB tokens from T0 on; k_of(j, kk): the operand of tokens 16 j .. 16 j + 15; ksc, vsc: their scales (e4m3 only, the
-  // score scale included in the first); v: the rows of V in LDS.  More tokens at a time give the wave independent work for
-  // the latencies of the products and exponentials.
+  // 16 SUB tokens from T0 on; k_of(j, kk): the operand of tokens 16 j .. 16 j + 15; scales: theirs in LDS (e4m3 only); v: the
+  // rows of V in LDS.  More tokens at a time give the wave independent work for the latencies of the products and exponentials.
   template <int SUB, typename F>
-  __device__ __forceinline__ void step(const SharedArgs& a, int T0, bool edge, F k_of, const float* ksc, const float* vsc, const bf16x8* v) {
+  __device__ __forceinline__ void step(const SharedArgs& a, int T0, bool edge, F k_of, const Scales scales, const bf16x8* v) {
     typedef typename S::P P;
     constexpr int N = 4 * SUB;
     const int lane = threadIdx.x & 63, r = lane & 15, grp = lane >> 4;
@@ -339,8 +353,15 @@ template <typename T, bool FP8, int D> struct QueryBlock {
       f32x4 st = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kk = 0; kk < S::KK; ++kk) st = HalfMfma<T>::run(k_of(j, kk), q[kk], st);
+      if constexpr (FP8) {
+        const f32x4 k4 = *reinterpret_cast<const f32x4*>(scales.k + 16 * j + 4 * grp);
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(scales.log_v + 16 * j + 4 * grp);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * j + i] = FP8 ? st[i] * ksc[4 * j + i] : st[i];
+        for (int i = 0; i < 4; ++i) s[4 * j + i] = fmaf(st[i], k4[i], l4[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * j + i] = st[i];
+      }
     }
     if (edge) {
 #pragma unroll
@@ -363,12 +384,26 @@ template <typename T, bool FP8, int D> struct QueryBlock {
     }
     const float ref = m == -kInf ? 0.f : m;   // nothing seen yet: every score here is masked, p = 0
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    typename S::pvec pf[SUB / 2];
+    typename S::pvec pf[SUB / 2], rest[FP8 ? 1 : SUB / 2];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float p = __builtin_amdgcn_exp2f(FP8 ? s[i] - ref : fmaf(s[i], a.scale_log2e, -ref));
-      sum[i & 3] += p;
-      pf[i >> 3][i & 7] = (P)(FP8 ? p * vsc[i] : p);
+    for (int j = 0; j < SUB; ++j) {
+      f32x4 r4;
+      if constexpr (FP8) r4 = *reinterpret_cast<const f32x4*>(scales.inverse_v + 16 * j + 4 * grp);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int half = j >> 1, at = 4 * (j & 1) + i;
+        if constexpr (FP8) {
+          const float w = __builtin_amdgcn_exp2f(s[4 * j + i] - ref);
+          sum[i] = fmaf(w, r4[i], sum[i]);
+          pf[half][at] = (P)w;
+        } else {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], a.scale_log2e, -ref));
+          sum[i] += p;
+          const P high = (P)p;
+          pf[half][at] = high;
+          rest[half][at] = (P)(p - (float)high);
+        }
+      }
     }
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     // tokens 4 grp + i and 16 + 4 grp + i (of each 32) of dim 16 dd + r: the order P holds them in
@@ -385,7 +420,9 @@ template <typename T, bool FP8, int D> struct QueryBlock {
         }
         typedef short s16x8 __attribute__((ext_vector_type(8)));
         const s16x8 both = {piece[0][0], piece[0][1], piece[0][2], piece[0][3], piece[1][0], piece[1][1], piece[1][2], piece[1][3]};
-        o[dd] = HalfMfma<P>::run(__builtin_bit_cast(typename S::pvec, both), pf[half], o[dd]);
+        const auto vt = __builtin_bit_cast(typename S::pvec, both);
+        o[dd] = HalfMfma<P>::run(vt, pf[half], o[dd]);
+        if constexpr (!FP8) o[dd] = HalfMfma<P>::run(vt, rest[half], o[dd]);
       }
     }
   }
@@ -504,27 +541,17 @@ template <typename T, bool FP8, bool PAGED, int D, int THREADS, int TOKENS, bool
       stage<typename S::P, FP8, D>(rows, row_of(i) - FIRST * THREADS / S::ROW16, piece_of(i), w);
     }
   }
-  __device__ __forceinline__ void stage_scales(const Raw& x, float* k_scale, float* v_scale) const {
+  __device__ __forceinline__ void stage_scales(const Raw& x, const Scales to) const {
     if constexpr (NS == 2) {
-      if (thread < TOKENS) { k_scale[thread] = x.s[0] * a.scale_log2e; v_scale[thread] = x.s[1]; }
+      if (thread < TOKENS) { to.k[thread] = x.s[0] * a.scale_log2e; to.set_v(thread, x.s[1]); }
     }
     if constexpr (NS == 1) {
-      if (thread < TOKENS) k_scale[thread] = x.s[0] * a.scale_log2e;
-      else if (thread < 2 * TOKENS) v_scale[thread - TOKENS] = x.s[0];
+      if (thread < TOKENS) to.k[thread] = x.s[0] * a.scale_log2e;
+      else if (thread < 2 * TOKENS) to.set_v(thread - TOKENS, x.s[0]);
     }
   }
 };
 
-// The scales of the lane's 4 SUB tokens of a step.
-template <int SUB> __device__ __forceinline__ void read_scales(const float* k_scale, const float* v_scale, int grp, float* ksc, float* vsc) {
-#pragma unroll
-  for (int j = 0; j < SUB; ++j) {
-    const f32x4 k4 = *reinterpret_cast<const f32x4*>(k_scale + 16 * j + 4 * grp);
-    const f32x4 v4 = *reinterpret_cast<const f32x4*>(v_scale + 16 * j + 4 * grp);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { ksc[4 * j + i] = k4[i]; vsc[4 * j + i] = v4[i]; }
-  }
-}
 // A wave's smallest limit: from there on its scores need the mask.
 __device__ __forceinline__ int wave_least(int limit) {
 #pragma unroll
@@ -544,8 +571,7 @@ __device__ __forceinline__ void block_item(const SharedArgs& a, const i32x4 r0, 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, grp = lane >> 4;
   bf16x8* const lds_k = lds + wave * 2 * kStep * S::KC;
   bf16x8* const lds_v = lds_k + kStep * S::KC;
-  float* const k_scale = lds_scale + wave * 128;
-  float* const v_scale = k_scale + 64;
+  const Scales scales{lds_scale + wave * 192, lds_scale + wave * 192 + 64, lds_scale + wave * 192 + 128};
   const int t0 = r1[0] + (LONG ? wave * TOKENS : 0), t1 = r1[1];
   History<PAGED> history(a, PAGED && !r1[3] ? r0[0] : r1[2], h);
   typedef Rows<T, FP8, PAGED, D, 64, TOKENS, true> Tile;
@@ -565,16 +591,14 @@ __device__ __forceinline__ void block_item(const SharedArgs& a, const i32x4 r0, 
         wave_sync();
         tile.template stage_k<PART * COUNT, COUNT>(now, lds_k);
         tile.template stage_v<PART * COUNT, COUNT>(now, T0, lds_v);
-        if constexpr (FP8 && PART == 0) tile.stage_scales(now, k_scale, v_scale);
+        if constexpr (FP8 && PART == 0) tile.stage_scales(now, scales);
         wave_sync();
         if constexpr (PART == PARTS - 1) tile.fetch(T0 + STRIDE, raw);
-        float ksc[8], vsc[8];
-        if constexpr (FP8) read_scales<2>(k_scale + kStep * PART, v_scale + kStep * PART, grp, ksc, vsc);
         if (PART == 0 || from < t1)
           block.template step<2>(a, from, from + kStep > least, [&](int j, int kk) {
             const int tok = 16 * j + r;
             return __builtin_bit_cast(typename S::kvec, lds_k[tok * S::KC + ((4 * kk + grp) ^ (tok & (S::KC - 1)))]);
-          }, ksc, vsc, lds_v);
+          }, scales + kStep * PART, lds_v);
       };
       part(std::integral_constant<int, 0>{});
       if constexpr (PARTS == 2) part(std::integral_constant<int, 1>{});
@@ -631,8 +655,7 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const i32x4 r0,
   typedef Shape<T, FP8, D> S;
   bf16x8* const lds_k = lds;
   bf16x8* const lds_v = lds + kShareTile * S::KC;
-  float* const k_scale = lds_scale;
-  float* const v_scale = lds_scale + kShareTile;
+  const Scales scales{lds_scale, lds_scale + kShareTile, lds_scale + 2 * kShareTile};
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, grp = lane >> 4;
   const int t0 = r1[0], t1 = r1[1];
   const int q0 = r0[2] * kQueryTile, blocks = (min(r0[1] * a.G - q0, kQueryTile) + 15) / 16;
@@ -656,19 +679,17 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const i32x4 r0,
       __syncthreads();
       tile.template stage_k<0, Tile::N>(raw, lds_k);
       tile.template stage_v<0, Tile::N>(raw, T0, lds_v);
-      if constexpr (FP8) tile.stage_scales(raw, k_scale, v_scale);
+      if constexpr (FP8) tile.stage_scales(raw, scales);
       __syncthreads();
       tile.fetch(T0 + kShareTile, raw);
       if (busy) {
         for (int part = first; part < first + count; ++part) {
           const int row = STEP * part, from = T0 + row;
           if (from >= t1) break;
-          float ksc[4 * SUB], vsc[4 * SUB];
-          if constexpr (FP8) read_scales<SUB>(k_scale + row, v_scale + row, grp, ksc, vsc);
           block.template step<SUB>(a, from, from + STEP > least, [&](int j, int kk) {
             const int tok = row + 16 * j + r;
             return __builtin_bit_cast(typename S::kvec, lds_k[tok * S::KC + ((4 * kk + grp) ^ (tok & (S::KC - 1)))]);
-          }, ksc, vsc, lds_v + row * S::KC);
+          }, scales + row, lds_v + row * S::KC);
         }
       }
     }
@@ -706,7 +727,7 @@ template <typename T, bool FP8, bool PAGED, int D>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3 : 2))) shared_attention_kernel(SharedArgs a) {
   typedef Shape<T, FP8, D> S;
   __shared__ bf16x8 lds[2 * kShareTile * S::KC];   // K and V: 32 tokens for each wave, or 128 for the workgroup
-  __shared__ __attribute__((aligned(16))) float lds_scale[4 * 128];
+  __shared__ __attribute__((aligned(16))) float lds_scale[4 * 192];
   static_assert(3 * 64 * (D / 4 + 2) * 4 <= (int)sizeof(lds), "the waves' results fit the tile memory");
   if (!list_fits(a, D)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
