@@ -57,51 +57,83 @@ struct ScheduleArgs {
 
 __device__ __forceinline__ int round_up(int v, int step) { return (v + step - 1) / step * step; }
 
-// Sums and exclusive prefix sums over 1024 threads.
-__device__ __forceinline__ int scan_1024(int v, int* scratch, int* total) {
+// Four sums, and four exclusive prefix sums with their totals, over 1024 threads.
+__device__ __forceinline__ f32x4 sum4_1024(f32x4 v, f32x4* scratch) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = wave_sum(v[i]);
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+  __syncthreads();
+  f32x4 t = scratch[0];
+#pragma unroll
+  for (int w = 1; w < 16; ++w) t += scratch[w];
+  return t;
+}
+__device__ __forceinline__ i32x4 scan4_1024(const i32x4 v, i32x4* scratch, i32x4* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
+  i32x4 x = v;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int up = __shfl_up(x, o, 64);
-    if (lane >= o) x += up;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int up = __shfl_up(x[i], o, 64);
+      if (lane >= o) x[i] += up;
+    }
   }
-  __syncthreads();
   if (lane == 63) scratch[wave] = x;
   __syncthreads();
-  int before = 0, all = 0;
+  i32x4 before = {0, 0, 0, 0}, all = {0, 0, 0, 0};
 #pragma unroll
   for (int w = 0; w < 16; ++w) {
-    before += w < wave ? scratch[w] : 0;
-    all += scratch[w];
+    const i32x4 t = scratch[w];
+    if (w < wave) before += t;
+    all += t;
   }
   *total = all;
   return before + x - v;
 }
-__device__ __forceinline__ float sum_1024(float v, float* scratch) { return block_sum<16>(v, scratch); }
 
+// One workgroup.  A thread has PER rows and PER groups (one each up to 1024 of them).  Its time is that of its dependent
+// rounds: everything is read from memory at the start, at once, and the sums and places of all kinds go through two joins.
+template <int PER>
 __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
-  constexpr int PER = kMaxRows / 1024;
-  __shared__ int starts[kMaxRows + 1], length[kMaxRows], extent[kMaxRows];
-  __shared__ int scratch[16];
-  __shared__ float fscratch[16];
-  const int tid = threadIdx.x, G = a.QH / a.KH;
-  const int capacity = (int)a.capacity;
-  for (int g = tid; g <= a.groups; g += 1024) {
-    const int s = a.starts[g];
-    starts[g] = s < 0 ? 0 : s > a.B ? a.B : s;
-    if (g < a.groups) extent[g] = 0;
+  constexpr int MOST = 1024 * PER;
+  __shared__ int starts[MOST + 1], extent[MOST], source[MOST], prefix[MOST];
+  __shared__ f32x4 fscratch[16];
+  __shared__ i32x4 scratch[16];
+  const int tid = threadIdx.x, G = a.QH / a.KH, capacity = (int)a.capacity;
+  int length[PER], slot_of[PER], group[PER], shared[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int b = tid * PER + i;
+    length[i] = slot_of[i] = 0;
+    if (b < a.B) {
+      const int position = a.positions[b];
+      slot_of[i] = a.slot_ids ? a.slot_ids[b] : b;
+      const bool on = (!a.active || a.active[b]) && slot_of[i] >= 0 && position >= 0;
+      length[i] = !on ? 0 : position < capacity ? position + 1 : capacity;
+    }
+    if (b < a.groups) {
+      const int s = a.starts[b], p = a.prefix_lengths[b];
+      starts[b] = s < 0 ? 0 : s > a.B ? a.B : s;
+      prefix[b] = p < 0 ? 0 : p > capacity ? capacity : p;
+      source[b] = a.prefix_slots[b];
+      extent[b] = 0;
+    }
+  }
+  if (tid == 0) {
+    const int s = a.starts[a.groups];
+    starts[a.groups] = s < 0 ? 0 : s > a.B ? a.B : s;
   }
   __syncthreads();
   // bounds out of order would give a row to several groups: such a list is marked as nobody's (its users return NaN)
   int disorder = 0;
-  for (int g = tid; g < a.groups; g += 1024) disorder |= starts[g] > starts[g + 1];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) disorder |= tid * PER + i < a.groups && starts[tid * PER + i] > starts[tid * PER + i + 1];
   if (__syncthreads_or(disorder)) {
     if (tid == 0) a.schedule[kHRows] = -1;
     return;
   }
   // a row's group: the last one that starts at or before it
-  int group[PER], shared[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int b = tid * PER + i;
@@ -113,14 +145,10 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
       const int mid = (lo + hi) >> 1;
       if (starts[mid] <= b) lo = mid; else hi = mid;
     }
-    int len = a.positions[b] < capacity ? a.positions[b] + 1 : capacity;
-    if (len < 0 || (a.active && !a.active[b]) || (a.slot_ids && a.slot_ids[b] < 0)) len = 0;
-    length[b] = len;
-    if (starts[lo] <= b && b < starts[lo + 1] && a.prefix_slots[lo] >= 0) {
-      const int p = a.prefix_lengths[lo];
+    if (starts[lo] <= b && b < starts[lo + 1] && source[lo] >= 0) {
       group[i] = lo;
-      shared[i] = p < 0 ? 0 : p > capacity ? capacity : p;
-      atomicMax(&extent[lo], len < shared[i] ? len : shared[i]);
+      shared[i] = prefix[lo];
+      atomicMax(&extent[lo], length[i] < shared[i] ? length[i] : shared[i]);   // what the group's rows see of it
     }
   }
   __syncthreads();
@@ -134,26 +162,26 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
     const int b = tid * PER + i;
     if (b >= a.B) continue;
     if (group[i] >= 0) (wide(group[i]) ? wide_tokens : other_tokens) += (float)extent[group[i]];
-    if (length[b] > shared[i]) {
-      other_tokens += (float)(length[b] - shared[i]);
-      other_work += (float)(length[b] - shared[i]) * (float)own_tiles;
+    if (length[i] > shared[i]) {
+      other_tokens += (float)(length[i] - shared[i]);
+      other_work += (float)(length[i] - shared[i]) * (float)own_tiles;
     }
   }
-  for (int g = tid; g < a.groups; g += 1024) {
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int g = tid * PER + i;
+    if (g >= a.groups) continue;
     if (wide(g)) wide_work += (float)extent[g] * (float)((queries(g) + kQueryTile - 1) / kQueryTile);
     else other_work += (float)extent[g];
   }
-  wide_tokens = sum_1024(wide_tokens, fscratch);
-  other_tokens = sum_1024(other_tokens, fscratch);
-  wide_work = sum_1024(wide_work, fscratch);
-  other_work = sum_1024(other_work, fscratch);
+  const f32x4 sums = sum4_1024(f32x4{wide_tokens, other_tokens, wide_work, other_work}, fscratch);
   auto chunk_of = [&](float tokens, float work, int items) {
     // a little more than the quotient: the sums are rounded
     const float need = fmaxf(tokens / (float)kSplitSlots, work * (float)a.KH / (float)items);
     return round_up((int)fminf(need * 1.0001f, 1.0e9f) + 1, kGrain);
   };
-  const int wide_chunk = chunk_of(wide_tokens, wide_work, kSharedItems);
-  const int other_chunk = chunk_of(other_tokens, other_work, kOwnItems);
+  const int wide_chunk = chunk_of(sums[0], sums[2], kSharedItems);
+  const int other_chunk = chunk_of(sums[1], sums[3], kOwnItems);
   // a part's chunks, and its records by kind (0 shared, 1 long, 2 short)
   struct Part { int chunk, chunks, records, kind; };
   auto shared_part = [&](int g) {
@@ -181,7 +209,7 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
     np[i] = ns[i] = 0;
     if (b < a.B) {
       if (group[i] >= 0) np[i] = shared_part(group[i]).chunks;
-      const Part own = own_part(length[b] - shared[i]);
+      const Part own = own_part(length[i] - shared[i]);
       ns[i] = own.chunks;
       slots += np[i] + ns[i];
       mine[1] += own.kind == 1 ? own.records : 0;
@@ -193,13 +221,9 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
       for (int k = 0; k < 3; ++k) mine[k] += part.kind == k ? part.records : 0;
     }
   }
-  int total, totals[3], at[3], before = 0;
-  int slot = scan_1024(slots, scratch, &total);
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    at[k] = before + scan_1024(mine[k], scratch, &totals[k]);
-    before += totals[k];
-  }
+  i32x4 totals;
+  const i32x4 first = scan4_1024(i32x4{mine[0], mine[1], mine[2], slots}, scratch, &totals);
+  int at[3] = {first[0], totals[0] + first[1], totals[0] + totals[1] + first[2]}, slot = first[3];
   int32_t* const records = a.schedule + kHeader + kRowInts * a.B;
   auto put = [&](const Part& part, int row, int rows, int tiles, int offset, int t0, int end, int source, int is_shared) {
     int& place = part.kind == 0 ? at[0] : part.kind == 1 ? at[1] : at[2];
@@ -214,13 +238,13 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
   for (int i = 0; i < PER; ++i) {
     const int b = tid * PER + i;
     if (b < a.B) {
-      *reinterpret_cast<i32x4*>(a.schedule + kHeader + kRowInts * b) = i32x4{slot, np[i], ns[i], length[b]};
+      *reinterpret_cast<i32x4*>(a.schedule + kHeader + kRowInts * b) = i32x4{slot, np[i], ns[i], length[i]};
       slot += np[i] + ns[i];
-      put(own_part(length[b] - shared[i]), b, 1, own_tiles, np[i], shared[i], length[b], a.slot_ids ? a.slot_ids[b] : b, 0);
+      put(own_part(length[i] - shared[i]), b, 1, own_tiles, np[i], shared[i], length[i], slot_of[i], 0);
     }
     if (b < a.groups) {
       const Part part = shared_part(b);
-      if (part.chunks) put(part, starts[b], starts[b + 1] - starts[b], part.records / part.chunks, 0, 0, extent[b], a.prefix_slots[b], 1);
+      if (part.chunks) put(part, starts[b], starts[b + 1] - starts[b], part.records / part.chunks, 0, 0, extent[b], source[b], 1);
     }
   }
   if (tid == 0) {
@@ -768,40 +792,50 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 6
 }
 
 // Joins the partial results of one (row, query head) per wave: weights 2^{m_c - max}, one chunk per lane, read back lane by
-// lane; lanes own dims.
+// lane; lanes own dims.  The results were written by other XCDs and come from beyond the local L2: what counts is the
+// number of dependent loads, so a chunk's maximum and sum are read together, and the results of eight chunks at a time.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) shared_combine_kernel(SharedArgs a) {
-  constexpr int PER = (D + 63) / 64;
+  constexpr int PER = (D + 63) / 64, BATCH = 8;
   const int lane = threadIdx.x & 63, b = blockIdx.x, qh = blockIdx.y * 4 + (threadIdx.x >> 6);
   if (qh >= a.QH) return;
   T* out = (T*)a.out + ((int64_t)b * a.QH + qh) * D;
+  const i32x4 row = *reinterpret_cast<const i32x4*>(a.schedule + kHeader + kRowInts * b);
   if (!list_fits(a, D)) {   // a work list of another batch
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       if (lane + 64 * i < D) out[lane + 64 * i] = Elem<T>::store(__builtin_nanf(""));
     return;
   }
-  const i32x4 row = *reinterpret_cast<const i32x4*>(a.schedule + kHeader + kRowInts * b);
   const int n = row[3] > 0 ? row[1] + row[2] : 0;
   const int64_t first = (int64_t)row[0] * a.QH + qh;
-  float top = -kInf;
-  for (int c = lane; c < n; c += 64) top = fmaxf(top, a.m[first + (int64_t)c * a.QH]);
-  top = wave_max(top);
-  float lt = 0.f, o[PER] = {};
+  float top = -kInf, lt = 0.f, o[PER] = {};
   for (int c0 = 0; c0 < n; c0 += 64) {
-    const int c = c0 + lane;
-    float f = 0.f;
-    if (c < n) {
-      const float mc = a.m[first + (int64_t)c * a.QH], lc = a.l[first + (int64_t)c * a.QH];
-      f = top == -kInf ? 1.f : __builtin_amdgcn_exp2f(mc - top);
-      lt = fmaf(lc, f, lt);
-    }
     const int here = min(64, n - c0);
-    for (int i = 0; i < here; ++i) {
-      const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
+    const int64_t mine = first + (int64_t)(c0 + min(lane, here - 1)) * a.QH;
+    const float mc = lane < here ? a.m[mine] : -kInf, lc = a.l[mine];
+    const float now = fmaxf(top, wave_max(mc)), before = now == -kInf ? 1.f : __builtin_amdgcn_exp2f(top - now);
+    const float f = lane >= here ? 0.f : now == -kInf ? 1.f : __builtin_amdgcn_exp2f(mc - now);
+    lt = lt * before + (lane < here ? lc * f : 0.f);
+    top = now;
 #pragma unroll
-      for (int u = 0; u < PER; ++u)
-        if (lane + 64 * u < D) o[u] = fmaf(a.acc[(first + (int64_t)(c0 + i) * a.QH) * D + lane + 64 * u], w, o[u]);
+    for (int u = 0; u < PER; ++u) o[u] *= before;
+    for (int i0 = 0; i0 < here; i0 += BATCH) {
+      float v[BATCH][PER];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const float* from = a.acc + (first + (int64_t)(c0 + min(i0 + i, here - 1)) * a.QH) * D;
+#pragma unroll
+        for (int u = 0; u < PER; ++u) v[i][u] = from[min(lane + 64 * u, D - 1)];
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        // chunks past the last: weight 0, of a value that was read before and is not used
+        const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(i0 + i, 63)));
+#pragma unroll
+        for (int u = 0; u < PER; ++u)
+          if (i0 + i < here) o[u] = fmaf(v[i][u], w, o[u]);
+      }
     }
   }
   lt = wave_sum(lt);
@@ -843,7 +877,8 @@ int lfm2_shared_schedule(int32_t* schedule, const int32_t* positions, const uint
   LFM2_REQUIRE(groups > 0 && groups <= kMaxRows, "shared_schedule: 1 to %d groups", kMaxRows);
   LFM2_REQUIRE(starts && prefix_slots && prefix_lengths, "shared_schedule: the groups need bounds, slots and lengths");
   const ScheduleArgs a{schedule, positions, slot_ids, starts, prefix_slots, prefix_lengths, active, capacity, (int)B, (int)groups, QH, KH, D};
-  hipLaunchKernelGGL(shared_schedule_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
+  if (B <= 1024 && groups <= 1024) hipLaunchKernelGGL(shared_schedule_kernel<1>, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL(shared_schedule_kernel<kMaxRows / 1024>, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
   LFM2_LAUNCH_CHECK();
 }
 

@@ -242,6 +242,8 @@ def test_large_scores_keep_their_order(ops):
 def test_many_rows_and_a_long_history(ops):
     Batch([(40, 700, 0)] * 3 + [(1, 9, 0)] * 70, (1, 5, 64), heads=(4, 1), seed=12).check(ops)
     Batch([(2, 20000, 0)], (3, 9000), heads=(4, 1), seed=13, fp8=True).check(ops)
+    Batch([(1, 9, 0), (2, 3, 0)] * 520 + [(30, 40, 0)], (1, 5), heads=(2, 1), dim=32, seed=20).check(ops)   # more than 1024 rows and groups
+    Batch([(2, 9, 0)] * 600, (1, 140), heads=(2, 1), dim=32, seed=21).check(ops)
 
 
 def test_bad_slots_pages_bounds_and_foreign_schedules_give_nan(ops):
