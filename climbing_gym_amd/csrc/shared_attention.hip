@@ -180,7 +180,27 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
     const float need = fmaxf(tokens / (float)kSplitSlots, work * (float)a.KH / (float)items);
     return round_up((int)fminf(need * 1.0001f, 1.0e9f) + 1, kGrain);
   };
-  const int wide_chunk = chunk_of(sums[0], sums[2], kSharedItems);
+  // The shared parts' chunk: of sixteen sizes up to about twice the smallest that will do, the one whose longest workgroup is
+  // shortest (rounds of the workgroups times tokens, and what an item costs besides).  One wave tries one size.  (32 groups of
+  // 4 to 7 k tokens: 512 items of up to 3500 tokens instead of 640 of 2816, two rounds for a quarter of the workgroups.)
+  const int smallest = chunk_of(sums[0], sums[2], kSharedItems), step = round_up(smallest / 16 + 1, kGrain);
+  {
+    const int wave = tid >> 6, chunk = smallest + wave * step;
+    int items = 0;
+    for (int g = tid & 63; g < a.groups; g += 64)
+      if (wide(g)) items += (extent[g] + chunk - 1) / chunk * ((queries(g) + kQueryTile - 1) / kQueryTile);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) items += __shfl_xor(items, o, 64);
+    if ((tid & 63) == 0) scratch[wave][0] = (items * a.KH + kSharedBlocks - 1) / kSharedBlocks * (chunk + kGrain);
+    __syncthreads();
+  }
+  int wide_chunk = smallest, least = scratch[0][0];
+#pragma unroll
+  for (int c = 1; c < 16; ++c) {
+    const int cost = scratch[c][0];
+    if (cost < least) { least = cost; wide_chunk = smallest + c * step; }
+  }
+  __syncthreads();
   const int other_chunk = chunk_of(sums[1], sums[3], kOwnItems);
   // a part's chunks, and its records by kind (0 shared, 1 long, 2 short)
   struct Part { int chunk, chunks, records, kind; };
@@ -364,93 +384,38 @@ template <typename T, bool FP8, int D> struct QueryBlock {
     for (int dd = 0; dd < D / 16; ++dd) o[dd] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // 16 SUB tokens from T0 on; k_of(j, kk): the operand of tokens 16 j .. 16 j + 15; scales: theirs in LDS (e4m3 only); v: the
-  // rows of V in LDS.  More tokens at a time give the wave independent work for the latencies of the products and exponentials.
-  template <int SUB, typename F>
-  __device__ __forceinline__ void step(const SharedArgs& a, int T0, bool edge, F k_of, const Scales scales, const bf16x8* v) {
-    typedef typename S::P P;
-    constexpr int N = 4 * SUB;
-    const int lane = threadIdx.x & 63, r = lane & 15, grp = lane >> 4;
-    float s[N];
+  __device__ __forceinline__ void raise(float top) {   // a new maximum of the query, the same in its four lanes
+    const float mnew = fmaxf(m, top);
+    const float alpha = mnew == -kInf ? 1.f : __builtin_amdgcn_exp2f(m - mnew);
+    m = mnew;
+    l *= alpha;
 #pragma unroll
-    for (int j = 0; j < SUB; ++j) {
-      f32x4 st = {0.f, 0.f, 0.f, 0.f};
+    for (int dd = 0; dd < D / 16; ++dd)
 #pragma unroll
-      for (int kk = 0; kk < S::KK; ++kk) st = HalfMfma<T>::run(k_of(j, kk), q[kk], st);
-      if constexpr (FP8) {
-        const f32x4 k4 = *reinterpret_cast<const f32x4*>(scales.k + 16 * j + 4 * grp);
-        const f32x4 l4 = *reinterpret_cast<const f32x4*>(scales.log_v + 16 * j + 4 * grp);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * j + i] = fmaf(st[i], k4[i], l4[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[4 * j + i] = st[i];
-      }
-    }
-    if (edge) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) s[i] = T0 + 16 * (i >> 2) + 4 * grp + (i & 3) < limit ? s[i] : -kInf;
-    }
-    float mx = s[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
-    if constexpr (!FP8) mx *= a.scale_log2e;   // the scale is positive: scores stay unscaled until the exponential
-    if (__any(mx > m + 8.0f)) {
-      mx = max_lane_xor32(max_lane_xor16(mx));
-      const float mnew = fmaxf(m, mx);
-      const float alpha = mnew == -kInf ? 1.f : __builtin_amdgcn_exp2f(m - mnew);
-      m = mnew;
-      l *= alpha;
-#pragma unroll
-      for (int dd = 0; dd < D / 16; ++dd)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[dd][i] *= alpha;
-    }
-    const float ref = m == -kInf ? 0.f : m;   // nothing seen yet: every score here is masked, p = 0
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    typename S::pvec pf[SUB / 2], rest[FP8 ? 1 : SUB / 2];
-#pragma unroll
-    for (int j = 0; j < SUB; ++j) {
-      f32x4 r4;
-      if constexpr (FP8) r4 = *reinterpret_cast<const f32x4*>(scales.inverse_v + 16 * j + 4 * grp);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int half = j >> 1, at = 4 * (j & 1) + i;
-        if constexpr (FP8) {
-          const float w = __builtin_amdgcn_exp2f(s[4 * j + i] - ref);
-          sum[i] = fmaf(w, r4[i], sum[i]);
-          pf[half][at] = (P)w;
-        } else {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * j + i], a.scale_log2e, -ref));
-          sum[i] += p;
-          const P high = (P)p;
-          pf[half][at] = high;
-          rest[half][at] = (P)(p - (float)high);
-        }
-      }
-    }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    // tokens 4 grp + i and 16 + 4 grp + i (of each 32) of dim 16 dd + r: the order P holds them in
-#pragma unroll
-    for (int dd = 0; dd < D / 16; ++dd) {
-#pragma unroll
-      for (int half = 0; half < SUB / 2; ++half) {
-        s16x4 piece[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int tok = 32 * half + 16 * j + 4 * grp + (r >> 2), c = 2 * dd + ((r & 3) >> 1);
-          const char* at = reinterpret_cast<const char*>(v + tok * S::KC + (c ^ (tok & (S::KC - 1)))) + 8 * (r & 1);
-          piece[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
-        }
-        typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const s16x8 both = {piece[0][0], piece[0][1], piece[0][2], piece[0][3], piece[1][0], piece[1][1], piece[1][2], piece[1][3]};
-        const auto vt = __builtin_bit_cast(typename S::pvec, both);
-        o[dd] = HalfMfma<P>::run(vt, pf[half], o[dd]);
-        if constexpr (!FP8) o[dd] = HalfMfma<P>::run(vt, rest[half], o[dd]);
-      }
-    }
+      for (int i = 0; i < 4; ++i) o[dd][i] *= alpha;
   }
-
+  // A wave's results to LDS, lane by lane, and another wave's joined to one's own.
+  static constexpr int kShare = 64 * (D / 4 + 2);   // floats
+  __device__ __forceinline__ void hand_over(float* to) const {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[(4 * dd + i) * 64 + lane] = o[dd][i];
+    to[D / 4 * 64 + lane] = m;
+    to[(D / 4 + 1) * 64 + lane] = l;
+  }
+  __device__ __forceinline__ void take_over(const float* from) {
+    const int lane = threadIdx.x & 63;
+    const float om = from[D / 4 * 64 + lane];
+    raise(om);
+    const float f = m == -kInf ? 1.f : __builtin_amdgcn_exp2f(om - m);
+    l = fmaf(from[(D / 4 + 1) * 64 + lane], f, l);
+#pragma unroll
+    for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[dd][i] = fmaf(from[(4 * dd + i) * 64 + lane], f, o[dd][i]);
+  }
   __device__ __forceinline__ void finish(bool bad) {   // row sums; a slot or page outside the cache makes them NaN
     l = add_lane_xor32(add_lane_xor16(l));
     if (bad) l = __builtin_nanf("");
@@ -463,6 +428,116 @@ template <typename T, bool FP8, int D> struct QueryBlock {
     if (grp == 0) { a.m[place] = m; a.l[place] = l; }
   }
 };
+
+// NB blocks of queries meet 16 SUB tokens from T0 on.  k: the rows of K in LDS, v: those of V, scales: their scales (e4m3
+// only).  What is read from LDS serves all blocks: with one block a wave the LDS is busy longer than the vector unit.
+template <typename T, bool FP8, int D, int SUB, int NB>
+__device__ __forceinline__ void attend_step(const SharedArgs& a, QueryBlock<T, FP8, D>* blocks, int T0, bool edge, const bf16x8* k,
+                                            const bf16x8* v, const Scales scales) {
+  typedef Shape<T, FP8, D> S;
+  typedef typename S::P P;
+  constexpr int N = 4 * SUB;
+  const int lane = threadIdx.x & 63, r = lane & 15, grp = lane >> 4;
+  float s[NB][N];
+#pragma unroll
+  for (int j = 0; j < SUB; ++j) {
+    const int tok = 16 * j + r;
+    f32x4 st[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) st[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < S::KK; ++kk) {
+      const auto kf = __builtin_bit_cast(typename S::kvec, k[tok * S::KC + ((4 * kk + grp) ^ (tok & (S::KC - 1)))]);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) st[n] = HalfMfma<T>::run(kf, blocks[n].q[kk], st[n]);
+    }
+    if constexpr (FP8) {
+      const f32x4 k4 = *reinterpret_cast<const f32x4*>(scales.k + 16 * j + 4 * grp);
+      const f32x4 l4 = *reinterpret_cast<const f32x4*>(scales.log_v + 16 * j + 4 * grp);
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][4 * j + i] = fmaf(st[n][i], k4[i], l4[i]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][4 * j + i] = st[n][i];
+    }
+  }
+  float mx[NB];
+  bool raise = false;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[n][i] = T0 + 16 * (i >> 2) + 4 * grp + (i & 3) < blocks[n].limit ? s[n][i] : -kInf;
+    }
+    mx[n] = s[n][0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) mx[n] = fmaxf(mx[n], s[n][i]);
+    if constexpr (!FP8) mx[n] *= a.scale_log2e;   // the scale is positive: scores stay unscaled until the exponential
+    raise |= mx[n] > blocks[n].m + 8.0f;
+  }
+  if (__any(raise)) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) blocks[n].raise(max_lane_xor32(max_lane_xor16(mx[n])));
+  }
+  typename S::pvec pf[NB][SUB / 2], rest[NB][FP8 ? 1 : SUB / 2];
+  float ref[NB], sum[NB][4];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    ref[n] = blocks[n].m == -kInf ? 0.f : blocks[n].m;   // nothing seen yet: every score here is masked, p = 0
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[n][i] = 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < SUB; ++j) {
+    f32x4 r4;
+    if constexpr (FP8) r4 = *reinterpret_cast<const f32x4*>(scales.inverse_v + 16 * j + 4 * grp);
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int half = j >> 1, at = 4 * (j & 1) + i;
+        if constexpr (FP8) {
+          const float w = __builtin_amdgcn_exp2f(s[n][4 * j + i] - ref[n]);
+          sum[n][i] = fmaf(w, r4[i], sum[n][i]);
+          pf[n][half][at] = (P)w;
+        } else {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[n][4 * j + i], a.scale_log2e, -ref[n]));
+          sum[n][i] += p;
+          const P high = (P)p;
+          pf[n][half][at] = high;
+          rest[n][half][at] = (P)(p - (float)high);
+        }
+      }
+  }
+#pragma unroll
+  for (int n = 0; n < NB; ++n) blocks[n].l += (sum[n][0] + sum[n][1]) + (sum[n][2] + sum[n][3]);
+  // tokens 4 grp + i and 16 + 4 grp + i (of each 32) of dim 16 dd + r: the order P holds them in
+#pragma unroll
+  for (int dd = 0; dd < D / 16; ++dd) {
+#pragma unroll
+    for (int half = 0; half < SUB / 2; ++half) {
+      s16x4 piece[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int tok = 32 * half + 16 * j + 4 * grp + (r >> 2), c = 2 * dd + ((r & 3) >> 1);
+        const char* at = reinterpret_cast<const char*>(v + tok * S::KC + (c ^ (tok & (S::KC - 1)))) + 8 * (r & 1);
+        piece[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+      }
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      const s16x8 both = {piece[0][0], piece[0][1], piece[0][2], piece[0][3], piece[1][0], piece[1][1], piece[1][2], piece[1][3]};
+      const auto vt = __builtin_bit_cast(typename S::pvec, both);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        blocks[n].o[dd] = HalfMfma<P>::run(vt, pf[n][half], blocks[n].o[dd]);
+        if constexpr (!FP8) blocks[n].o[dd] = HalfMfma<P>::run(vt, rest[n][half], blocks[n].o[dd]);
+      }
+    }
+  }
+}
 
 // Where the tokens of an item are.  Dense: base + t * c1; paged: through the table row.
 template <bool PAGED> struct History {
@@ -618,51 +693,21 @@ __device__ __forceinline__ void block_item(const SharedArgs& a, const i32x4 r0, 
         if constexpr (FP8 && PART == 0) tile.stage_scales(now, scales);
         wave_sync();
         if constexpr (PART == PARTS - 1) tile.fetch(T0 + STRIDE, raw);
-        if (PART == 0 || from < t1)
-          block.template step<2>(a, from, from + kStep > least, [&](int j, int kk) {
-            const int tok = 16 * j + r;
-            return __builtin_bit_cast(typename S::kvec, lds_k[tok * S::KC + ((4 * kk + grp) ^ (tok & (S::KC - 1)))]);
-          }, scales + kStep * PART, lds_v);
+        if (PART == 0 || from < t1) attend_step<T, FP8, D, 2, 1>(a, &block, from, from + kStep > least, lds_k, lds_v, scales + kStep * PART);
       };
       part(std::integral_constant<int, 0>{});
       if constexpr (PARTS == 2) part(std::integral_constant<int, 1>{});
     }
   }
   block.finish(__any(history.bad));
-  if constexpr (LONG) {   // the four results meet: each wave's O, m and l, lane by lane
+  if constexpr (LONG) {   // the four results meet
     float* const share = reinterpret_cast<float*>(lds);
-    constexpr int AREA = 64 * (D / 4 + 2);
     __syncthreads();
-    if (wave > 0) {
-      float* const to = share + (wave - 1) * AREA;
-#pragma unroll
-      for (int dd = 0; dd < D / 16; ++dd)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) to[(4 * dd + i) * 64 + lane] = block.o[dd][i];
-      to[D / 4 * 64 + lane] = block.m;
-      to[(D / 4 + 1) * 64 + lane] = block.l;
-    }
+    if (wave > 0) block.hand_over(share + (wave - 1) * block.kShare);
     __syncthreads();
     if (wave == 0) {
-      float mw[4], mm = block.m;
-      mw[0] = block.m;
 #pragma unroll
-      for (int w = 1; w < 4; ++w) { mw[w] = share[(w - 1) * AREA + D / 4 * 64 + lane]; mm = fmaxf(mm, mw[w]); }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) mw[w] = mm == -kInf ? 1.f : __builtin_amdgcn_exp2f(mw[w] - mm);
-      block.m = mm;
-      block.l *= mw[0];
-#pragma unroll
-      for (int w = 1; w < 4; ++w) block.l = fmaf(share[(w - 1) * AREA + (D / 4 + 1) * 64 + lane], mw[w], block.l);
-#pragma unroll
-      for (int dd = 0; dd < D / 16; ++dd)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v = block.o[dd][i] * mw[0];
-#pragma unroll
-          for (int w = 1; w < 4; ++w) v = fmaf(share[(w - 1) * AREA + (4 * dd + i) * 64 + lane], mw[w], v);
-          block.o[dd][i] = v;
-        }
+      for (int w = 0; w < 3; ++w) block.take_over(share + w * block.kShare);
       block.store(a);
     }
     __syncthreads();   // the next item's tiles go where the results met
@@ -672,32 +717,37 @@ __device__ __forceinline__ void block_item(const SharedArgs& a, const i32x4 r0, 
 }
 
 // A shared item: up to 64 queries of a group against tokens [t0, t1) of one KV head, 128 tokens at a time.  All four waves
-// stage the tile (the next ones are on their way to registers meanwhile); then wave w takes query block w, or, with at most
-// two blocks, block w % 2 and half w / 2 of the tile's tokens, whose two results meet at the end.
+// stage the tile (the next one is on its way to registers meanwhile); then each takes NB query blocks against its share of the
+// tile's tokens: the waves of one set of blocks share them evenly, and their results meet at the end.  An e4m3 history takes
+// two blocks a wave (32 x 16 rows, 5500 shared tokens: 73 us against 79 with one), since each is read with three scales per
+// token; a 16-bit one takes one block and twice the tokens at a time (85 us against 90: the weights' second part and the
+// wider rows in flight need the registers).
 template <typename T, bool FP8, bool PAGED, int D>
 __device__ __forceinline__ void shared_item(const SharedArgs& a, const i32x4 r0, const i32x4 r1, int h, bf16x8* lds, float* lds_scale) {
   typedef Shape<T, FP8, D> S;
+  typedef QueryBlock<T, FP8, D> Block;
+  constexpr int NB = FP8 ? 2 : 1, SUB = FP8 || D > 64 ? 2 : 4, STEP = 16 * SUB;
   bf16x8* const lds_k = lds;
   bf16x8* const lds_v = lds + kShareTile * S::KC;
   const Scales scales{lds_scale, lds_scale + kShareTile, lds_scale + 2 * kShareTile};
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, grp = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t0 = r1[0], t1 = r1[1];
-  const int q0 = r0[2] * kQueryTile, blocks = (min(r0[1] * a.G - q0, kQueryTile) + 15) / 16;
-  const bool halves = blocks <= 2;
-  const int mine = halves ? wave & 1 : wave;
-  const bool busy = mine < blocks;
+  const int q0 = r0[2] * kQueryTile, queries = min(r0[1] * a.G - q0, kQueryTile);
+  const int sets = (queries > 32 ? 4 : 2) / NB, set = wave & (sets - 1);
+  const int tokens = kShareTile / 4 * sets, first = wave / sets * tokens;   // the wave's share of a tile
   History<PAGED> history(a, r1[2], h);
   typedef Rows<T, FP8, PAGED, D, 256, kShareTile, false> Tile;
   Tile tile(a, history, t1, threadIdx.x);
   typename Tile::Raw raw;
   const bool readable = PAGED || !history.bad;
   if (readable) tile.fetch(t0, raw);
-  QueryBlock<T, FP8, D> block;
-  block.start(a, r0, t1, h, q0 + 16 * mine);
-  if (!busy) block.place = -1;
-  const int least = wave_least(block.limit);
-  constexpr int SUB = D <= 64 ? 4 : 2, STEP = 16 * SUB, STEPS = kShareTile / STEP;
-  const int first = halves ? STEPS / 2 * (wave >> 1) : 0, count = halves ? STEPS / 2 : STEPS;   // the wave's steps of a tile
+  Block blocks[NB];
+  int least = t1;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    blocks[n].start(a, r0, t1, h, q0 + 16 * (NB * set + n));
+    least = min(least, wave_least(blocks[n].limit));
+  }
   if (readable) {
     for (int T0 = t0; T0 < t1; T0 += kShareTile) {
       __syncthreads();
@@ -706,45 +756,34 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const i32x4 r0,
       if constexpr (FP8) tile.stage_scales(raw, scales);
       __syncthreads();
       tile.fetch(T0 + kShareTile, raw);
-      if (busy) {
-        for (int part = first; part < first + count; ++part) {
-          const int row = STEP * part, from = T0 + row;
-          if (from >= t1) break;
-          block.template step<SUB>(a, from, from + STEP > least, [&](int j, int kk) {
-            const int tok = row + 16 * j + r;
-            return __builtin_bit_cast(typename S::kvec, lds_k[tok * S::KC + ((4 * kk + grp) ^ (tok & (S::KC - 1)))]);
-          }, scales + row, lds_v + row * S::KC);
-        }
+      for (int row = first; row < first + tokens; row += STEP) {
+        const int from = T0 + row;
+        if (from >= t1) break;
+        attend_step<T, FP8, D, SUB, NB>(a, blocks, from, from + STEP > least, lds_k + row * S::KC, lds_v + row * S::KC, scales + row);
       }
     }
   }
-  block.finish(__syncthreads_or(history.bad));   // also: the last tile has been read by all waves
-  if (halves) {   // waves 2 and 3 hand their results to waves 0 and 1
-    float* const other = reinterpret_cast<float*>(lds) + (wave & 1) * 64 * (D / 4 + 2);   // lane by lane: O, then m and l
-    if (wave >= 2) {
+  const bool bad = __syncthreads_or(history.bad);   // also: the last tile has been read by all waves
 #pragma unroll
-      for (int dd = 0; dd < D / 16; ++dd)
+  for (int n = 0; n < NB; ++n) blocks[n].finish(bad);
+  // the first wave of a set keeps; the others hand over to it, one after the other
+  float* const share = reinterpret_cast<float*>(lds) + set * NB * Block::kShare;
+  for (int giver = sets; giver < 4; giver += sets) {
+    if (wave / sets == giver / sets) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) other[(4 * dd + i) * 64 + lane] = block.o[dd][i];
-      other[D / 4 * 64 + lane] = block.m;
-      other[(D / 4 + 1) * 64 + lane] = block.l;
+      for (int n = 0; n < NB; ++n) blocks[n].hand_over(share + n * Block::kShare);
     }
     __syncthreads();
-    if (wave < 2) {
-      const float om = other[D / 4 * 64 + lane], mm = fmaxf(block.m, om);
-      const float fa = mm == -kInf ? 1.f : __builtin_amdgcn_exp2f(block.m - mm), fb = mm == -kInf ? 1.f : __builtin_amdgcn_exp2f(om - mm);
-      block.l = block.l * fa + other[(D / 4 + 1) * 64 + lane] * fb;
-      block.m = mm;
+    if (wave < sets) {
 #pragma unroll
-      for (int dd = 0; dd < D / 16; ++dd)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) block.o[dd][i] = fmaf(other[(4 * dd + i) * 64 + lane], fb, block.o[dd][i] * fa);
-    } else {
-      block.place = -1;
+      for (int n = 0; n < NB; ++n) blocks[n].take_over(share + n * Block::kShare);
     }
+    __syncthreads();   // the next results, and the next item's tiles, go to the same place
   }
-  block.store(a);
-  __syncthreads();   // the next item's tiles go where the halves met
+  if (wave < sets) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) blocks[n].store(a);
+  }
 }
 
 template <typename T, bool FP8, bool PAGED, int D>
@@ -752,7 +791,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 6
   typedef Shape<T, FP8, D> S;
   __shared__ bf16x8 lds[2 * kShareTile * S::KC];   // K and V: 32 tokens for each wave, or 128 for the workgroup
   __shared__ __attribute__((aligned(16))) float lds_scale[4 * 192];
-  static_assert(3 * 64 * (D / 4 + 2) * 4 <= (int)sizeof(lds), "the waves' results fit the tile memory");
+  static_assert(4 * QueryBlock<T, FP8, D>::kShare * 4 <= (int)sizeof(lds), "the waves' results fit the tile memory");
   if (!list_fits(a, D)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int32_t* const records = a.schedule + kHeader + kRowInts * a.B;
