@@ -20,7 +20,10 @@ constexpr int kTurn = 256;                // workgroups, one per CU
 constexpr int kSharedBlocks = 2 * kTurn, kOtherBlocks = 3 * kTurn;
 constexpr int kSharedItems = 512;      // items the shared parts are cut into, if their length allows ...
 constexpr int kOwnItems = 2048;         // ... and the others
-constexpr int kWaveTokens = 128;      // up to this many tokens an item is one wave's
+// Up to this many tokens an item is one wave's, beyond it a workgroup's.  A workgroup's waves read four tiles in a row, which
+// the memory likes, and pay for their join.  512 rows with own parts of 256 / 500 / 1000 tokens: e4m3 46 / 70 / 125 us as
+// wave items, 55 / 79 / 127 as workgroup items; bf16 58 / 100 / 191 against 62 / 100 / 185; 256 rows of 2000: 176 against 169.
+constexpr int kWaveTokens = 1024;
 
 // ---- the work list (int32), built once per decode step and used by every attention layer
 //   header: what the list was built for, number of records of each of the three kinds of item
