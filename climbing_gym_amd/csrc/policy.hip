@@ -4,6 +4,10 @@
 #include "lfm2_common.h"
 
 namespace {
+#ifndef GT
+#define GT 512
+#define GV 16
+#endif
 
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_huge_valf();
@@ -63,7 +67,11 @@ template <bool ENTROPY, int N> __device__ __forceinline__ void add_values(RowSta
 
 // Statistics of a whole row, the same in every thread: threads keep their own maximum and sums (four 16-byte loads in
 // flight each), which are joined once at the end.
-template <typename T, int THREADS, bool ENTROPY>
+template <bool STREAM, typename V> __device__ __forceinline__ V load_row(const V* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <typename T, int THREADS, bool ENTROPY, bool STREAM>
 __device__ __forceinline__ RowStats row_stats(const T* __restrict__ row, int64_t V, float k, float* scratch) {
   constexpr int VE = RowVec<T>::N;
   typedef typename RowVec<T>::type vec;
@@ -73,7 +81,7 @@ __device__ __forceinline__ RowStats row_stats(const T* __restrict__ row, int64_t
   for (; i + 3 * THREADS < nvec; i += 4 * THREADS) {
     vec v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const vec*>(row + (i + j * THREADS) * VE);
+    for (int j = 0; j < 4; ++j) v[j] = load_row<STREAM>(reinterpret_cast<const vec*>(row + (i + j * THREADS) * VE));
     float z[4 * VE];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -82,7 +90,7 @@ __device__ __forceinline__ RowStats row_stats(const T* __restrict__ row, int64_t
     add_values<ENTROPY, 4 * VE>(a, z, k);
   }
   for (; i < nvec; i += THREADS) {
-    const vec v = *reinterpret_cast<const vec*>(row + i * VE);
+    const vec v = load_row<STREAM>(reinterpret_cast<const vec*>(row + i * VE));
     float z[VE];
 #pragma unroll
     for (int e = 0; e < VE; ++e) z[e] = (float)v[e];
@@ -126,7 +134,7 @@ struct LogprobArgs {
 };
 
 // One workgroup per row; reads the row once.  stats[row] = (max, log s, entropy, 0) for the gradient.
-template <typename T, int THREADS, bool ENTROPY>
+template <typename T, int THREADS, bool ENTROPY, bool STREAM>
 __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) {
   __shared__ float scratch[THREADS / 64];
   const int64_t row = blockIdx.x, target = a.targets[row];
@@ -143,7 +151,7 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
   const float t = row_temperature(a.temperatures, a.temperature, row);
   const bool in_range = target < a.V;
   const float zt = (float)z[in_range ? target : 0];
-  const RowStats st = row_stats<T, THREADS, ENTROPY>(z, a.V, LFM2_LOG2E / t, scratch);
+  const RowStats st = row_stats<T, THREADS, ENTROPY, STREAM>(z, a.V, LFM2_LOG2E / t, scratch);
   if (threadIdx.x == 0) {
     const RowResult r = finish_row(st, zt, in_range, t);
     a.logprobs[row] = r.logprob;
@@ -157,18 +165,27 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) 
 
 // d/dz_v of g logp(target) + h H = (g ([v = target] - p_v) - h p_v (log p_v + H)) / T for N consecutive elements, the
 // first of which is `first`; c holds what is the same along the row.
-struct GradRow { float m, k, log2_s, g, h, entropy, inv_t; int64_t target; };
+struct GradRow { float m, k, log2_s, g, h, entropy, inv_t, scale; int64_t target; };   // scale = -g / T
 template <typename T, int N, bool ENTROPY>
 __device__ __forceinline__ void grad_values(const GradRow& c, const float* z, int64_t first, T* out) {
+  const int64_t hot = c.target - first;
+  float v[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const float d = fmaxf(fmaf(z[i] - c.m, c.k, -c.log2_s), -1.0e30f);   // log2 p
+    const float d = fmaf(z[i] - c.m, c.k, -c.log2_s);   // log2 p
     const float p = __builtin_amdgcn_exp2f(d);
-    const float inner = ENTROPY ? fmaf(c.h, fmaf(d, kLn2, c.entropy), c.g) : c.g;
-    float v = -p * inner;
-    if (first + i == c.target) v += c.g;
-    out[i] = Elem<T>::store(v * c.inv_t);
+    if constexpr (ENTROPY) {
+      v[i] = -p * fmaf(c.h, fmaf(fmaxf(d, -1.0e30f), kLn2, c.entropy), c.g) * c.inv_t;   // 0 * -inf has no place in the sum
+    } else {
+      v[i] = p * c.scale;
+    }
   }
+  if (hot >= 0 && hot < N) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = fmaf(i == hot ? c.g : 0.f, c.inv_t, v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = Elem<T>::store(v[i]);
 }
 __device__ __forceinline__ GradRow grad_row(float m, float log_s, float entropy, float g, float h, float temperature,
                                             int64_t target, int64_t V) {
@@ -184,6 +201,7 @@ __device__ __forceinline__ GradRow grad_row(float m, float log_s, float entropy,
   c.g = log_s == log_s && target < V ? g : __builtin_nanf("");
   c.target = target;
   if (m == -kInf && log_s == -kInf) { c.g = 0.f; c.h = 0.f; c.m = 0.f; c.log2_s = 0.f; c.entropy = 0.f; }   // no finite logit: no gradient
+  c.scale = -c.g * c.inv_t;
   return c;
 }
 
@@ -485,19 +503,31 @@ struct GradientArgs {
   float temperature, grad_scale;
 };
 
-// One workgroup per row: statistics, the token's loss slope, and the row's gradient.
-template <typename T, int THREADS, bool ENTROPY>
+// Keeps the compiler from holding a row's values unpacked (twice the registers of 16-bit ones) from one sweep to the next.
+template <typename V, int N> __device__ __forceinline__ void forget_unpacked(V (&held)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    i32x4 raw = __builtin_bit_cast(i32x4, held[j]);
+    asm volatile("" : "+v"(raw));
+    held[j] = __builtin_bit_cast(V, raw);
+  }
+}
+
+// One workgroup per row: statistics, the token's loss slope, and the row's gradient.  VECS > 0: the row is read once and
+// waits in registers (16 bytes each) while its statistics are joined; 0: a row too long for that is read twice.
+template <typename T, int THREADS, int VECS, bool ENTROPY>
 __global__ void __launch_bounds__(THREADS) policy_gradient_kernel(GradientArgs a) {
   constexpr int VE = RowVec<T>::N;
   typedef typename RowVec<T>::type vec;
   __shared__ float scratch[THREADS / 64];
   __shared__ int iscratch[THREADS / 64];
-  const int64_t row = blockIdx.x, nvec = a.V / VE;
+  const int64_t row = blockIdx.x, nvec = a.V / VE, tail = nvec * VE + threadIdx.x;
+  const bool has_tail = tail < a.V;
   T* out = (T*)a.grad + row * a.grad_stride;
   if (!token_counts(a.loss, row)) {
     const vec zero = {};
     for (int64_t i = threadIdx.x; i < nvec; i += THREADS) *reinterpret_cast<vec*>(out + i * VE) = zero;
-    if (threadIdx.x < a.V - nvec * VE) out[nvec * VE + threadIdx.x] = Elem<T>::store(0.f);
+    if (has_tail) out[tail] = Elem<T>::store(0.f);
     if (threadIdx.x == 0) {
       a.logprobs[row] = 0.f;
       if (a.entropy) a.entropy[row] = 0.f;
@@ -506,41 +536,85 @@ __global__ void __launch_bounds__(THREADS) policy_gradient_kernel(GradientArgs a
   }
   const int64_t target = a.loss.targets[row];
   const T* z = (const T*)a.logits + row * a.stride;
-  const float t = row_temperature(a.temperatures, a.temperature, row);
+  vec held[VECS > 0 ? VECS : 1];
+  if constexpr (VECS > 0) {
+#pragma unroll
+    for (int j = 0; j < VECS; ++j) {
+      const int64_t i = threadIdx.x + (int64_t)j * THREADS;
+      if (i < nvec) held[j] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(z + i * VE));
+    }
+  }
+  const float t = row_temperature(a.temperatures, a.temperature, row), k = LFM2_LOG2E / t;
   const bool in_range = target < a.V;
   const float zt = (float)z[in_range ? target : 0];
-  const RowStats st = row_stats<T, THREADS, ENTROPY>(z, a.V, LFM2_LOG2E / t, scratch);
+  const float zl = has_tail ? (float)z[tail] : -kInf;
+  // while the row is on its way: the token's weight
   Totals total = partial_totals(a.loss, threadIdx.x, THREADS);
   total.tokens = block_sum_int<THREADS / 64>(total.tokens, iscratch);
   total.sequences = block_sum_int<THREADS / 64>(total.sequences, iscratch);
-  const RowResult r = finish_row(st, zt, in_range, t);
   const int64_t s = a.loss.cu ? sequence_of(a.loss.cu, 0, a.loss.S, row) : 0;
   const float w = token_weight(a.loss, total, a.loss.aggregate == LFM2_MEAN_SEQUENCES && a.loss.cu ? sequence_count(a.loss, s) : 0);
-  const TokenTerms term = token_terms(a.loss, r.logprob, a.loss.old[row], a.loss.ref ? a.loss.ref[row] : 0.f,
-                                      a.loss.advantages[a.loss.per_sequence ? s : row]);
+  const float old = a.loss.old[row], ref = a.loss.ref ? a.loss.ref[row] : 0.f, advantage = a.loss.advantages[a.loss.per_sequence ? s : row];
+  RowStats st;
+  if constexpr (VECS > 0) {
+    float mx = zl;
+#pragma unroll
+    for (int j = 0; j < VECS; ++j)
+      if (threadIdx.x + (int64_t)j * THREADS < nvec) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) mx = fmaxf(mx, (float)held[j][e]);
+      }
+    forget_unpacked(held);
+    st.m = group_max<THREADS>(mx, scratch);
+    const float base = st.m == -kInf ? 0.f : st.m;   // nothing but -inf (or NaN): the exponentials are 0 (or NaN)
+    float sum = 0.f, u = 0.f;
+    auto add = [&](float x) {
+      const float d = (x - base) * k, e = __builtin_amdgcn_exp2f(d);
+      sum += e;
+      if (ENTROPY) u = fmaf(e, fmaxf(d, -1.0e30f), u);
+    };
+#pragma unroll
+    for (int j = 0; j < VECS; ++j)
+      if (threadIdx.x + (int64_t)j * THREADS < nvec) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) add((float)held[j][e]);
+      }
+    if (has_tail) add(zl);
+    st.u = ENTROPY ? group_sum<THREADS>(u, scratch) : 0.f;
+    st.s = group_sum<THREADS>(sum, scratch);
+  } else {
+    st = row_stats<T, THREADS, ENTROPY, false>(z, a.V, k, scratch);
+  }
+  const RowResult r = finish_row(st, zt, in_range, t);
+  const TokenTerms term = token_terms(a.loss, r.logprob, old, ref, advantage);
   if (threadIdx.x == 0) {
     a.logprobs[row] = r.logprob;
     if (ENTROPY) a.entropy[row] = r.entropy;
   }
   const GradRow c = grad_row(st.m, r.log_s, ENTROPY ? r.entropy : 0.f, a.grad_scale * w * term.slope,
                              ENTROPY ? -a.grad_scale * a.loss.entropy_coef * w : 0.f, t, target, a.V);
-  for (int64_t i = threadIdx.x; i < nvec; i += THREADS) {
-    const vec v = *reinterpret_cast<const vec*>(z + i * VE);
+  auto store = [&](int64_t i, const vec v) {
     float x[VE];
     T y[VE];
 #pragma unroll
     for (int e = 0; e < VE; ++e) x[e] = (float)v[e];
     grad_values<T, VE, ENTROPY>(c, x, i * VE, y);
-    vec w8;
+    vec o;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) w8[e] = y[e];
-    *reinterpret_cast<vec*>(out + i * VE) = w8;
+    for (int e = 0; e < VE; ++e) o[e] = y[e];
+    *reinterpret_cast<vec*>(out + i * VE) = o;
+  };
+  if constexpr (VECS > 0) {
+    forget_unpacked(held);
+#pragma unroll
+    for (int j = 0; j < VECS; ++j) {
+      const int64_t i = threadIdx.x + (int64_t)j * THREADS;
+      if (i < nvec) store(i, held[j]);
+    }
+  } else {
+    for (int64_t i = threadIdx.x; i < nvec; i += THREADS) store(i, *reinterpret_cast<const vec*>(z + i * VE));
   }
-  if (threadIdx.x < a.V - nvec * VE) {
-    const int64_t tail = nvec * VE + threadIdx.x;
-    const float x = (float)z[tail];
-    grad_values<T, 1, ENTROPY>(c, &x, tail, out + tail);
-  }
+  if (has_tail) grad_values<T, 1, ENTROPY>(c, &zl, tail, out + tail);
 }
 
 // ===================================================================================== host side
@@ -567,6 +641,10 @@ int fill_loss(const char* name, LossArgs* a, const float* logprobs, const float*
                 __builtin_log1p((double)clip_high), dual_clip > 0.f ? __builtin_log((double)dual_clip) : 0.0};
   return LFM2_OK;
 }
+
+// Logits of this size or more leave the last-level cache (256 MB) before anybody reads them again: the scoring pass then
+// loads them with the non-temporal hint; smaller ones stay there for the gradient.
+constexpr int64_t kStreamBytes = 192ll << 20;
 
 int64_t count_slots(int64_t N, int64_t S, bool cu) { return cu ? S : (N + kCountBlock - 1) / kCountBlock; }
 int64_t loss_blocks(int64_t N) { return (N + kLossTokens - 1) / kLossTokens; }
@@ -608,14 +686,18 @@ int lfm2_token_logprobs(float* logprobs, float* entropy, float* stats, const voi
   LFM2_REQUIRE(temperatures || temperature > 0.f, "token_logprobs: temperature must be positive");
   const LogprobArgs a{logprobs, entropy, stats, logits, targets, temperatures, row_stride, V, temperature};
   hipStream_t s = (hipStream_t)stream;
+#define LOGPROBS_(THREADS, ENTROPY, STREAM) \
+  hipLaunchKernelGGL((token_logprobs_kernel<T, THREADS, ENTROPY, STREAM>), dim3((unsigned)N), dim3(THREADS), 0, s, a)
   DISPATCH_LOGITS(dtype, "token_logprobs",
+    const bool stream_once = N * row_stride * (int64_t)sizeof(T) >= kStreamBytes;
     if (V <= 8192) {
-      if (entropy) hipLaunchKernelGGL((token_logprobs_kernel<T, 128, true>), dim3((unsigned)N), dim3(128), 0, s, a);
-      else hipLaunchKernelGGL((token_logprobs_kernel<T, 128, false>), dim3((unsigned)N), dim3(128), 0, s, a);
+      if (stream_once) { if (entropy) LOGPROBS_(128, true, true); else LOGPROBS_(128, false, true); }
+      else { if (entropy) LOGPROBS_(128, true, false); else LOGPROBS_(128, false, false); }
     } else {
-      if (entropy) hipLaunchKernelGGL((token_logprobs_kernel<T, 512, true>), dim3((unsigned)N), dim3(512), 0, s, a);
-      else hipLaunchKernelGGL((token_logprobs_kernel<T, 512, false>), dim3((unsigned)N), dim3(512), 0, s, a);
+      if (stream_once) { if (entropy) LOGPROBS_(512, true, true); else LOGPROBS_(512, false, true); }
+      else { if (entropy) LOGPROBS_(512, true, false); else LOGPROBS_(512, false, false); }
     })
+#undef LOGPROBS_
   LFM2_LAUNCH_CHECK();
 }
 
@@ -688,9 +770,18 @@ int lfm2_policy_gradient(float* loss, float* stats, float* logprobs, float* entr
   hipStream_t s = (hipStream_t)stream;
   const LossWorkspace ws = split_workspace(workspace, N);
   launch_counts(&g.loss, ws.counts, s);
+#define GRADIENT_(THREADS, VECS)                                                                                                  \
+  do {                                                                                                                            \
+    if (entropy) hipLaunchKernelGGL((policy_gradient_kernel<T, THREADS, VECS, true>), dim3((unsigned)N), dim3(THREADS), 0, s, g);  \
+    else hipLaunchKernelGGL((policy_gradient_kernel<T, THREADS, VECS, false>), dim3((unsigned)N), dim3(THREADS), 0, s, g);         \
+  } while (0)
   DISPATCH_LOGITS(dtype, "policy_gradient",
-    if (entropy) hipLaunchKernelGGL((policy_gradient_kernel<T, 512, true>), dim3((unsigned)N), dim3(512), 0, s, g);
-    else hipLaunchKernelGGL((policy_gradient_kernel<T, 512, false>), dim3((unsigned)N), dim3(512), 0, s, g);)
+    const int64_t pieces = V / RowVec<T>::N;
+    if (pieces <= 256 * 4) GRADIENT_(256, 4);
+    else if (pieces <= 512 * 8) GRADIENT_(512, 8);
+    else if (pieces <= GT * GV) GRADIENT_(GT, GV);
+    else GRADIENT_(512, 0);)
+#undef GRADIENT_
   launch_loss(g.loss, nullptr, nullptr, ws, loss, stats, s);
   LFM2_LAUNCH_CHECK();
 }
