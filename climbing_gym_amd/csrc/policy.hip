@@ -4,10 +4,6 @@
 #include "lfm2_common.h"
 
 namespace {
-#ifndef GT
-#define GT 512
-#define GV 16
-#endif
 
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_huge_valf();
@@ -397,54 +393,50 @@ __global__ void __launch_bounds__(256) policy_count_kernel(int32_t* counts, Loss
 // order, so the result does not depend on how workgroups are scheduled.
 constexpr int kLossTerms = 6;          // policy, kl, entropy, cut, ratio, excess
 constexpr int kLossTokens = 1024;      // tokens per workgroup of 256 threads
-template <int THREADS>
-__device__ __forceinline__ void policy_tokens(const LossArgs& a, int64_t begin, int64_t end, float* grad, float* grad_entropy,
-                                              double* out, int* tokens_out) {
-  constexpr int WAVES = THREADS / 64;
-  __shared__ int counts[WAVES];
-  __shared__ double sums[WAVES][kLossTerms];
-  Totals total = partial_totals(a, threadIdx.x, THREADS);
-  total.tokens = block_sum_int<WAVES>(total.tokens, counts);
-  total.sequences = block_sum_int<WAVES>(total.sequences, counts);
-  double sum[kLossTerms] = {};
-  int64_t s_first = 0, s_last = 0;
-  if (a.cu && begin < end) {   // the same in every thread: the sequences this range of tokens meets
-    s_first = sequence_of(a.cu, 0, a.S, begin);
-    s_last = sequence_of(a.cu, s_first, a.S, end - 1);
+// What a token brings, read before anything is known about its weight (a token that does not count is read and not used).
+struct TokenInputs {
+  float logprob, old, ref, entropy, advantage;
+  bool counts;
+  __device__ __forceinline__ void read(const LossArgs& a, int64_t t, int64_t end) {
+    counts = t < end;
+    if (!counts) return;
+    logprob = a.logprobs[t];
+    old = a.old[t];
+    if (a.ref) ref = a.ref[t];
+    if (a.entropy) entropy = a.entropy[t];
+    if (!a.per_sequence) advantage = a.advantages[t];
+    counts = (!a.mask || a.mask[t]) && (!a.targets || a.targets[t] >= 0);
   }
-  for (int64_t t = begin + threadIdx.x; t < end; t += THREADS) {
-    float g = 0.f, gh = 0.f;
-    if (token_counts(a, t)) {
-      const int64_t s = a.cu ? sequence_of(a.cu, s_first, s_last + 1, t) : 0;
-      const float w = token_weight(a, total, a.aggregate == LFM2_MEAN_SEQUENCES && a.cu ? sequence_count(a, s) : 0);
-      const TokenTerms term = token_terms(a, a.logprobs[t], a.old[t], a.ref ? a.ref[t] : 0.f, a.advantages[a.per_sequence ? s : t]);
-      g = w * term.slope;
-      gh = -a.entropy_coef * w;
-      sum[0] += (double)w * term.policy;
-      sum[1] += (double)w * term.kl;
-      if (a.entropy) sum[2] += (double)w * a.entropy[t];
-      sum[3] += term.cut;
-      sum[4] += term.ratio;
-      sum[5] += term.excess;
+};
+struct TermSums {
+  double v[kLossTerms] = {};
+  // a token of sequence s with weight w: returns its gradient
+  __device__ __forceinline__ float add(const LossArgs& a, const TokenInputs& x, int64_t s, float w) {
+    const TokenTerms term = token_terms(a, x.logprob, x.old, x.ref, a.per_sequence ? a.advantages[s] : x.advantage);
+    v[0] += (double)w * term.policy;
+    v[1] += (double)w * term.kl;
+    if (a.entropy) v[2] += (double)w * x.entropy;
+    v[3] += term.cut;
+    v[4] += term.ratio;
+    v[5] += term.excess;
+    return w * term.slope;
+  }
+  // over the workgroup, to out[kLossTerms] (valid after the next barrier)
+  template <int WAVES> __device__ __forceinline__ void join(double (*scratch)[kLossTerms], double* out) const {
+#pragma unroll
+    for (int i = 0; i < kLossTerms; ++i) {
+      const double x = wave_sum_double(v[i]);
+      if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6][i] = x;
     }
-    if (grad) grad[t] = g;
-    if (grad_entropy) grad_entropy[t] = gh;
-  }
+    __syncthreads();
+    if (threadIdx.x < kLossTerms) {
+      double x = 0.0;
 #pragma unroll
-  for (int i = 0; i < kLossTerms; ++i) {
-    const double v = wave_sum_double(sum[i]);
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6][i] = v;
+      for (int i = 0; i < WAVES; ++i) x += scratch[i][threadIdx.x];
+      out[threadIdx.x] = x;
+    }
   }
-  __syncthreads();
-  if (threadIdx.x < kLossTerms) {
-    double v = 0.0;
-#pragma unroll
-    for (int i = 0; i < WAVES; ++i) v += sums[i][threadIdx.x];
-    out[threadIdx.x] = v;
-  }
-  *tokens_out = total.tokens;
-}
-
+};
 // loss, then (policy, kl, entropy, share cut, mean ratio, mean of r - 1 - log r, tokens) from the summed terms.
 __device__ __forceinline__ void store_loss(const LossArgs& a, const double* sum, int tokens, float* loss, float* stats) {
   const double n = tokens > 0 ? tokens : 1;
@@ -460,13 +452,51 @@ __device__ __forceinline__ void store_loss(const LossArgs& a, const double* sum,
 
 __global__ void __launch_bounds__(256)
 policy_tokens_kernel(LossArgs a, float* grad, float* grad_entropy, double* partials, int* tokens) {
-  __shared__ double out[kLossTerms];
-  const int64_t begin = (int64_t)blockIdx.x * kLossTokens;
-  int total;
-  policy_tokens<256>(a, begin, clamp_token(begin + kLossTokens, a.N), grad, grad_entropy, out, &total);
+  __shared__ i32x4 counts[4];
+  __shared__ double scratch[4][kLossTerms], out[kLossTerms];
+  constexpr int PER = kLossTokens / 256;
+  const int64_t begin = (int64_t)blockIdx.x * kLossTokens, end = clamp_token(begin + kLossTokens, a.N);
+  TokenInputs inputs[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) inputs[i].read(a, begin + threadIdx.x + 256 * i, end);
+  const int64_t cu_first = a.cu ? a.cu[0] : 0, cu_last = a.cu ? a.cu[a.S] : a.N;
+  // one sweep over the sequences: the totals, and how many start at or before this range's first and last token
+  i32x4 n = {0, 0, 0, 0};
+  for (int64_t s = threadIdx.x; s < a.ncounts; s += 256) {
+    const int here = sequence_count(a, s);
+    n[0] += here;
+    n[1] += here > 0;
+    if (a.cu) {
+      n[2] += a.cu[s] <= begin;
+      n[3] += a.cu[s] < end;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) n[i] = wave_sum_int(n[i]);
+  if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = n;
+  __syncthreads();
+  n = (counts[0] + counts[1]) + (counts[2] + counts[3]);
+  const Totals total{n[0], n[1]};
+  const int64_t s_first = n[2] > 0 ? n[2] - 1 : 0, s_last = n[3] > 0 ? n[3] - 1 : 0;
+  TermSums sums;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int64_t t = begin + threadIdx.x + 256 * i;
+    if (t >= end) continue;
+    float g = 0.f, gh = 0.f;
+    if (inputs[i].counts && t >= cu_first && t < cu_last) {   // not behind the last sequence
+      const int64_t s = a.cu ? sequence_of(a.cu, s_first, s_last + 1, t) : 0;
+      const float w = token_weight(a, total, a.aggregate == LFM2_MEAN_SEQUENCES && a.cu ? sequence_count(a, s) : 0);
+      g = sums.add(a, inputs[i], s, w);
+      gh = -a.entropy_coef * w;
+    }
+    if (grad) grad[t] = g;
+    if (grad_entropy) grad_entropy[t] = gh;
+  }
+  sums.join<4>(scratch, out);
   __syncthreads();
   if (threadIdx.x < kLossTerms) partials[(int64_t)blockIdx.x * kLossTerms + threadIdx.x] = out[threadIdx.x];
-  if (blockIdx.x == 0 && threadIdx.x == 0) *tokens = total;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *tokens = total.tokens;
 }
 __global__ void __launch_bounds__(256)
 policy_finish_kernel(LossArgs a, const double* partials, const int* tokens, int64_t blocks, float* loss, float* stats) {
@@ -483,13 +513,58 @@ policy_finish_kernel(LossArgs a, const double* partials, const int* tokens, int6
   __syncthreads();
   if (threadIdx.x == 0) store_loss(a, out, *tokens, loss, stats);
 }
-// Few tokens: the sums of the one workgroup are the batch's.
+// Few tokens and sequences: one workgroup counts, weighs and sums everything; the bounds and counts are in LDS.
+constexpr int kSingleTokens = 4096, kSingleSequences = 2048;
 __global__ void __launch_bounds__(1024) policy_single_kernel(LossArgs a, float* grad, float* grad_entropy, float* loss, float* stats) {
-  __shared__ double out[kLossTerms];
-  int total;
-  policy_tokens<1024>(a, 0, a.N, grad, grad_entropy, out, &total);
+  constexpr int PER = kSingleTokens / 1024;
+  __shared__ int bounds[kSingleSequences + 1], counts[kSingleSequences], iscratch[16];
+  __shared__ double scratch[16][kLossTerms], out[kLossTerms];
+  const int tid = threadIdx.x, S = a.cu ? (int)a.S : 1;
+  for (int s = tid; s <= S; s += 1024) {
+    bounds[s] = a.cu ? (int)clamp_token(a.cu[s], a.N) : s ? (int)a.N : 0;
+    if (s < S) counts[s] = 0;
+  }
+  TokenInputs inputs[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) inputs[i].read(a, tid + 1024 * i, a.N);
   __syncthreads();
-  if (threadIdx.x == 0) store_loss(a, out, total, loss, stats);
+  int sequence[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = tid + 1024 * i;
+    sequence[i] = 0;
+    if (!inputs[i].counts) continue;
+    if (t < bounds[0] || t >= bounds[S]) { inputs[i].counts = false; continue; }   // behind the last sequence
+    int lo = 0, hi = S;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (bounds[mid] <= t) lo = mid; else hi = mid;
+    }
+    sequence[i] = lo;
+    atomicAdd(&counts[lo], 1);
+  }
+  __syncthreads();
+  Totals total{0, 0};
+  for (int s = tid; s < S; s += 1024) { total.tokens += counts[s]; total.sequences += counts[s] > 0; }
+  total.tokens = block_sum_int<16>(total.tokens, iscratch);
+  total.sequences = block_sum_int<16>(total.sequences, iscratch);
+  TermSums sums;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int64_t t = tid + 1024 * i;
+    if (t >= a.N) continue;
+    float g = 0.f, gh = 0.f;
+    if (inputs[i].counts) {
+      const float w = token_weight(a, total, counts[sequence[i]]);
+      g = sums.add(a, inputs[i], sequence[i], w);
+      gh = -a.entropy_coef * w;
+    }
+    if (grad) grad[t] = g;
+    if (grad_entropy) grad_entropy[t] = gh;
+  }
+  sums.join<16>(scratch, out);
+  __syncthreads();
+  if (tid == 0) store_loss(a, out, total.tokens, loss, stats);
 }
 
 // ===================================================================================== loss and gradient from the logits
@@ -662,9 +737,9 @@ void launch_counts(LossArgs* a, int* counts, hipStream_t s) {
   hipLaunchKernelGGL(policy_count_kernel, dim3((unsigned)a->ncounts), dim3(256), 0, s, counts, *a);
   a->counts = counts;
 }
-constexpr int64_t kSingleTokens = 4096;   // up to here one workgroup does the whole loss
+bool single_workgroup(const LossArgs& a) { return a.N <= kSingleTokens && a.S <= kSingleSequences; }
 void launch_loss(const LossArgs& a, float* grad, float* grad_entropy, const LossWorkspace& ws, float* loss, float* stats, hipStream_t s) {
-  if (a.N <= kSingleTokens) {
+  if (single_workgroup(a)) {
     hipLaunchKernelGGL(policy_single_kernel, dim3(1), dim3(1024), 0, s, a, grad, grad_entropy, loss, stats);
     return;
   }
@@ -744,7 +819,7 @@ int lfm2_policy_loss(float* loss, float* stats, float* grad_logprobs, float* gra
   LFM2_REQUIRE(loss && stats && logprobs && workspace, "policy_loss: null argument");
   hipStream_t s = (hipStream_t)stream;
   const LossWorkspace ws = split_workspace(workspace, N);
-  launch_counts(&a, ws.counts, s);
+  if (!single_workgroup(a)) launch_counts(&a, ws.counts, s);
   launch_loss(a, grad_logprobs, grad_entropy, ws, loss, stats, s);
   LFM2_LAUNCH_CHECK();
 }
@@ -779,7 +854,7 @@ int lfm2_policy_gradient(float* loss, float* stats, float* logprobs, float* entr
     const int64_t pieces = V / RowVec<T>::N;
     if (pieces <= 256 * 4) GRADIENT_(256, 4);
     else if (pieces <= 512 * 8) GRADIENT_(512, 8);
-    else if (pieces <= GT * GV) GRADIENT_(GT, GV);
+    else if (pieces <= 512 * 16) GRADIENT_(512, 16);
     else GRADIENT_(512, 0);)
 #undef GRADIENT_
   launch_loss(g.loss, nullptr, nullptr, ws, loss, stats, s);

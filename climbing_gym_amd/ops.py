@@ -9,6 +9,7 @@ into a HIP graph.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -49,6 +50,9 @@ def _one_device(*tensors):
         reject(device is not None and t.device != device, "all tensors of a call live on one device")
         device = t.device
     return device
+
+
+_size = lru_cache(maxsize=1024)(query)   # sizes of workspaces: functions of the shapes alone
 
 
 def _call_on(device, name: str, *args) -> None:
@@ -579,7 +583,7 @@ def shared_schedule(positions, prefix: SharedPrefix, active=None, slot_ids=None,
     prefix.check()
     device = _one_device(positions, prefix.starts, prefix.slots, prefix.lengths, active, slot_ids)
     reject(query_heads <= 0 or kv_heads <= 0 or query_heads % kv_heads, "query heads must be a multiple of the KV heads")
-    size = query("lfm2_shared_schedule_size", rows, int(capacity), query_heads, kv_heads, head_dim)
+    size = _size("lfm2_shared_schedule_size", rows, int(capacity), query_heads, kv_heads, head_dim)
     schedule = torch.empty(max(size, 4), device=device, dtype=torch.int32)
     _call_on(device, "lfm2_shared_schedule", schedule, positions, active, slot_ids, prefix.starts, prefix.slots, prefix.lengths,
              rows, prefix.slots.numel(), int(capacity), query_heads, kv_heads, head_dim)
@@ -623,9 +627,9 @@ def attend_shared(q, k_cache, v_cache, k_scales, v_scales, positions, prefix: Sh
         schedule = shared_schedule(positions, prefix, active, slot_ids, capacity=capacity, query_heads=query_heads, kv_heads=heads, head_dim=dim)
     else:
         reject(schedule.dtype != torch.int32 or not schedule.is_contiguous()
-               or schedule.numel() < query("lfm2_shared_schedule_size", rows, capacity, query_heads, heads, dim),
+               or schedule.numel() < _size("lfm2_shared_schedule_size", rows, capacity, query_heads, heads, dim),
                "schedule must come from shared_schedule for this batch")
-    ws = torch.empty(query("lfm2_shared_attention_workspace", rows, capacity, query_heads, heads, dim), device=device, dtype=torch.float32)
+    ws = torch.empty(_size("lfm2_shared_attention_workspace", rows, capacity, query_heads, heads, dim), device=device, dtype=torch.float32)
     out = torch.empty_like(q)
     _call_on(device, "lfm2_shared_attention", out, q, k_cache, v_cache, k_scales, v_scales, schedule, block_table,
              0 if block_table is None else block_table.size(1), int(page), ws, rows, query_heads, heads, dim, capacity, pools, *strides,
@@ -986,7 +990,7 @@ def policy_loss_forward(logprobs: torch.Tensor, old_logprobs: torch.Tensor, adva
         return (torch.zeros((), device=device), torch.zeros(7, device=device), fresh(0), None if entropy is None else fresh(0))
     loss, stats, grad = fresh(), fresh(7), fresh(tokens)
     grad_entropy = None if entropy is None else fresh(tokens)
-    workspace = fresh(query("lfm2_policy_workspace", tokens, sequences, int(cu_seqlens is not None)))
+    workspace = fresh(_size("lfm2_policy_workspace", tokens, sequences, int(cu_seqlens is not None)))
     _call_on(device, "lfm2_policy_loss", loss, stats, grad, grad_entropy, logprobs, old_logprobs, advantages, ref_logprobs, entropy,
              mask, cu_seqlens, workspace, tokens, sequences, int(per_sequence), *config._arguments())
     return loss, stats, grad, grad_entropy
@@ -1038,7 +1042,7 @@ def policy_gradient(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: t
         return torch.zeros((), device=device), torch.zeros(7, device=device), fresh(0), grad
     loss, stats, logprobs = fresh(), fresh(7), fresh(tokens)
     entropies = fresh(tokens) if config.entropy_coef != 0.0 else None
-    workspace = fresh(query("lfm2_policy_workspace", tokens, sequences, int(cu_seqlens is not None)))
+    workspace = fresh(_size("lfm2_policy_workspace", tokens, sequences, int(cu_seqlens is not None)))
     _call_on(device, "lfm2_policy_gradient", loss, stats, logprobs, entropies, grad, _row_stride(grad), logits, _row_stride(logits),
              targets, old_logprobs, advantages, ref_logprobs, mask, cu_seqlens, temperatures, value, workspace, tokens,
              logits.size(1), sequences, int(per_sequence), *config._arguments(), float(grad_scale), _code(logits.dtype))
