@@ -29,12 +29,15 @@ constexpr int kWaveTokens = 1024;
 //   header: what the list was built for, number of records of each of the three kinds of item
 //   one record per row: first partial result, shared chunks, own chunks, length (0: sits out)
 //   one record per item, kind after kind: first row, rows, query tile, place of the partial result among the row's, first
-//   token, end token, slot or table row that holds them, 1 for a part that a group shares
+//   token, end token, slot or table row that holds them, whose tokens they are (kOwn, kShared, kCut)
 // A group with more queries than a block has its shared part cut into "shared" items, of a workgroup and up to 64 queries.
 // Everything else (rows' own parts, the shared parts of smaller groups) becomes items of one block of queries: a workgroup's
 // ("long"), or a wave's ("short") where the part has at most kWaveTokens tokens.
 enum { kHShared, kHLong, kHShort, kHRows, kHCapacity, kHQueryHeads, kHKvHeads, kHDim, kHeader = 16 };
 constexpr int kRowInts = 4, kRecordInts = 8;
+// A row that ends inside its group's prefix takes no part in the shared items: it would meet the tokens behind its end with
+// weight 0, and 0 times an infinity there is not 0.  It reads its piece of the prefix by itself (kCut).
+enum { kOwn, kShared, kCut };
 
 struct SlotBounds { int64_t slots, records; };
 // Upper bounds of the partial results and of the items of a batch, from what the host knows.  A row has at most
@@ -104,7 +107,8 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
   __shared__ f32x4 fscratch[16];
   __shared__ i32x4 scratch[16];
   const int tid = threadIdx.x, G = a.QH / a.KH, capacity = (int)a.capacity;
-  int length[PER], slot_of[PER], group[PER], shared[PER];
+  int length[PER], slot_of[PER], group[PER], shared[PER];   // shared: positions a row has in common with its group, 0: none
+  bool cut[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int b = tid * PER + i;
@@ -142,6 +146,7 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
     const int b = tid * PER + i;
     group[i] = -1;
     shared[i] = 0;
+    cut[i] = false;
     if (b >= a.B) continue;
     int lo = 0, hi = a.groups;
     while (hi - lo > 1) {
@@ -149,9 +154,14 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
       if (starts[mid] <= b) lo = mid; else hi = mid;
     }
     if (starts[lo] <= b && b < starts[lo + 1] && source[lo] >= 0) {
-      group[i] = lo;
-      shared[i] = prefix[lo];
-      atomicMax(&extent[lo], length[i] < shared[i] ? length[i] : shared[i]);   // what the group's rows see of it
+      cut[i] = length[i] < prefix[lo];
+      if (cut[i]) {
+        slot_of[i] = source[lo];
+      } else {
+        group[i] = lo;
+        shared[i] = prefix[lo];
+        extent[lo] = prefix[lo];   // the same value from every row of the group
+      }
     }
   }
   __syncthreads();
@@ -179,9 +189,9 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
   }
   const f32x4 sums = sum4_1024(f32x4{wide_tokens, other_tokens, wide_work, other_work}, fscratch);
   auto chunk_of = [&](float tokens, float work, int items) {
-    // a little more than the quotient: the sums are rounded
+    // a little more than the quotient: the sums are rounded.  (6e8 is above 2^40 tokens over kSplitSlots, and twice it an int.)
     const float need = fmaxf(tokens / (float)kSplitSlots, work * (float)a.KH / (float)items);
-    return round_up((int)fminf(need * 1.0001f, 1.0e9f) + 1, kGrain);
+    return round_up((int)fminf(need * 1.0001f, 6.0e8f) + 1, kGrain);
   };
   // The shared parts' chunk: of sixteen sizes up to about twice the smallest that will do, the one whose longest workgroup is
   // shortest (rounds of the workgroups times tokens, and what an item costs besides).  One wave tries one size.  (32 groups of
@@ -194,10 +204,10 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
       if (wide(g)) items += (extent[g] + chunk - 1) / chunk * ((queries(g) + kQueryTile - 1) / kQueryTile);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) items += __shfl_xor(items, o, 64);
-    if ((tid & 63) == 0) scratch[wave][0] = (items * a.KH + kSharedBlocks - 1) / kSharedBlocks * (chunk + kGrain);
+    if ((tid & 63) == 0) scratch[wave][0] = __builtin_bit_cast(int, (float)((items * a.KH + kSharedBlocks - 1) / kSharedBlocks) * (float)(chunk + kGrain));
     __syncthreads();
   }
-  int wide_chunk = smallest, least = scratch[0][0];
+  int wide_chunk = smallest, least = scratch[0][0];   // positive floats are in order as integers too
 #pragma unroll
   for (int c = 1; c < 16; ++c) {
     const int cost = scratch[c][0];
@@ -248,13 +258,13 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
   const i32x4 first = scan4_1024(i32x4{mine[0], mine[1], mine[2], slots}, scratch, &totals);
   int at[3] = {first[0], totals[0] + first[1], totals[0] + totals[1] + first[2]}, slot = first[3];
   int32_t* const records = a.schedule + kHeader + kRowInts * a.B;
-  auto put = [&](const Part& part, int row, int rows, int tiles, int offset, int t0, int end, int source, int is_shared) {
+  auto put = [&](const Part& part, int row, int rows, int tiles, int offset, int t0, int end, int source, int whose) {
     int& place = part.kind == 0 ? at[0] : part.kind == 1 ? at[1] : at[2];
     for (int c = 0; c < part.chunks; ++c)
       for (int qt = 0; qt < tiles; ++qt) {
         i32x4* r = reinterpret_cast<i32x4*>(records + (int64_t)kRecordInts * place++);
         r[0] = i32x4{row, rows, qt, offset + c};
-        r[1] = i32x4{t0 + c * part.chunk, min(t0 + (c + 1) * part.chunk, end), source, is_shared};
+        r[1] = i32x4{t0 + c * part.chunk, min(t0 + (c + 1) * part.chunk, end), source, whose};
       }
   };
 #pragma unroll
@@ -263,11 +273,11 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
     if (b < a.B) {
       *reinterpret_cast<i32x4*>(a.schedule + kHeader + kRowInts * b) = i32x4{slot, np[i], ns[i], length[i]};
       slot += np[i] + ns[i];
-      put(own_part(length[i] - shared[i]), b, 1, own_tiles, np[i], shared[i], length[i], slot_of[i], 0);
+      put(own_part(length[i] - shared[i]), b, 1, own_tiles, np[i], shared[i], length[i], slot_of[i], cut[i] ? kCut : kOwn);
     }
     if (b < a.groups) {
       const Part part = shared_part(b);
-      if (part.chunks) put(part, starts[b], starts[b + 1] - starts[b], part.records / part.chunks, 0, 0, extent[b], source[b], 1);
+      if (part.chunks) put(part, starts[b], starts[b + 1] - starts[b], part.records / part.chunks, 0, 0, extent[b], source[b], kShared);
     }
   }
   if (tid == 0) {
@@ -368,9 +378,9 @@ template <typename T, bool FP8, int D> struct QueryBlock {
   typename S::kvec q[S::KK];
   f32x4 o[D / 16];
   float m, l;
-  int limit, place;   // the query's last visible token + 1; row of the partial results, -1: nowhere
+  int place;   // row of the partial results, -1: nowhere
 
-  __device__ __forceinline__ void start(const SharedArgs& a, const i32x4 r0, int t1, int h, int q0) {
+  __device__ __forceinline__ void start(const SharedArgs& a, const i32x4 r0, int whose, int h, int q0) {
     const int lane = threadIdx.x & 63, r = lane & 15, grp = lane >> 4;
     const int row0 = r0[0], total = r0[1] * a.G, qi = min(q0 + r, total - 1);
     const int b = row0 + qi / a.G, head = h * a.G + qi % a.G;
@@ -378,9 +388,9 @@ template <typename T, bool FP8, int D> struct QueryBlock {
 #pragma unroll
     for (int kk = 0; kk < S::KK; ++kk) q[kk] = *reinterpret_cast<const typename S::kvec*>(src + 32 * kk + 8 * grp);
     const i32x4 record = *reinterpret_cast<const i32x4*>(a.schedule + kHeader + kRowInts * b);
-    const int len = record[3];
-    limit = len > 0 && len < t1 ? len : t1;   // a row that sits out computes something that is never stored
-    place = q0 + r < total && len > 0 ? (record[0] + r0[3]) * a.QH + head : -1;
+    // a row that sits out, or ends inside the prefix, computes something that is never stored
+    const bool mine = q0 + r < total && record[3] > 0 && (whose != kShared || r0[3] < record[1]);
+    place = mine ? (record[0] + r0[3]) * a.QH + head : -1;
     m = -kInf;
     l = 0.f;
 #pragma unroll
@@ -432,10 +442,10 @@ template <typename T, bool FP8, int D> struct QueryBlock {
   }
 };
 
-// NB blocks of queries meet 16 SUB tokens from T0 on.  k: the rows of K in LDS, v: those of V, scales: their scales (e4m3
+// NB blocks of queries meet 16 SUB tokens, of which the first `live` are the item's.  k: the rows of K in LDS, v: those of V, scales: their scales (e4m3
 // only).  What is read from LDS serves all blocks: with one block a wave the LDS is busy longer than the vector unit.
 template <typename T, bool FP8, int D, int SUB, int NB>
-__device__ __forceinline__ void attend_step(const SharedArgs& a, QueryBlock<T, FP8, D>* blocks, int T0, bool edge, const bf16x8* k,
+__device__ __forceinline__ void attend_step(const SharedArgs& a, QueryBlock<T, FP8, D>* blocks, int live, const bf16x8* k,
                                             const bf16x8* v, const Scales scales) {
   typedef Shape<T, FP8, D> S;
   typedef typename S::P P;
@@ -472,9 +482,9 @@ __device__ __forceinline__ void attend_step(const SharedArgs& a, QueryBlock<T, F
   bool raise = false;
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    if (edge) {
+    if (live < 16 * SUB) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) s[n][i] = T0 + 16 * (i >> 2) + 4 * grp + (i & 3) < blocks[n].limit ? s[n][i] : -kInf;
+      for (int i = 0; i < N; ++i) s[n][i] = 16 * (i >> 2) + 4 * grp + (i & 3) < live ? s[n][i] : -kInf;
     }
     mx[n] = s[n][0];
 #pragma unroll
@@ -654,13 +664,6 @@ template <typename T, bool FP8, bool PAGED, int D, int THREADS, int TOKENS, bool
   }
 };
 
-// A wave's smallest limit: from there on its scores need the mask.
-__device__ __forceinline__ int wave_least(int limit) {
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) limit = min(limit, __shfl_xor(limit, o, 64));
-  return __builtin_amdgcn_readfirstlane(limit);
-}
-
 // An item of one block of queries against tokens [t0, t1) of one KV head.  A wave works by itself on tiles of 4 KiB of K and
 // of V (at least 32 tokens): the next one is on its way to registers while the rows of the current one pass through the
 // wave's own LDS, 32 tokens at a time.  The four waves of a workgroup share a long item, taking its tiles round robin (the
@@ -675,15 +678,14 @@ __device__ __forceinline__ void block_item(const SharedArgs& a, const i32x4 r0, 
   bf16x8* const lds_v = lds_k + kStep * S::KC;
   const Scales scales{lds_scale + wave * 192, lds_scale + wave * 192 + 64, lds_scale + wave * 192 + 128};
   const int t0 = r1[0] + (LONG ? wave * TOKENS : 0), t1 = r1[1];
-  History<PAGED> history(a, PAGED && !r1[3] ? r0[0] : r1[2], h);
+  History<PAGED> history(a, PAGED && r1[3] == kOwn ? r0[0] : r1[2], h);
   typedef Rows<T, FP8, PAGED, D, 64, TOKENS, true> Tile;
   Tile tile(a, history, t1, lane);
   typename Tile::Raw raw;
   const bool work = t0 < t1 && (PAGED || !history.bad);   // the same for the whole wave
   if (work) tile.fetch(t0, raw);
   QueryBlock<T, FP8, D> block;
-  block.start(a, r0, t1, h, r0[2] * kQueryBlock);
-  const int least = wave_least(block.limit);
+  block.start(a, r0, r1[3], h, r0[2] * kQueryBlock);
   if (work) {
     for (int T0 = t0; T0 < t1; T0 += STRIDE) {
       typename Tile::Raw now = raw;
@@ -696,7 +698,7 @@ __device__ __forceinline__ void block_item(const SharedArgs& a, const i32x4 r0, 
         if constexpr (FP8 && PART == 0) tile.stage_scales(now, scales);
         wave_sync();
         if constexpr (PART == PARTS - 1) tile.fetch(T0 + STRIDE, raw);
-        if (PART == 0 || from < t1) attend_step<T, FP8, D, 2, 1>(a, &block, from, from + kStep > least, lds_k, lds_v, scales + kStep * PART);
+        if (PART == 0 || from < t1) attend_step<T, FP8, D, 2, 1>(a, &block, t1 - from, lds_k, lds_v, scales + kStep * PART);
       };
       part(std::integral_constant<int, 0>{});
       if constexpr (PARTS == 2) part(std::integral_constant<int, 1>{});
@@ -745,12 +747,8 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const i32x4 r0,
   const bool readable = PAGED || !history.bad;
   if (readable) tile.fetch(t0, raw);
   Block blocks[NB];
-  int least = t1;
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    blocks[n].start(a, r0, t1, h, q0 + 16 * (NB * set + n));
-    least = min(least, wave_least(blocks[n].limit));
-  }
+  for (int n = 0; n < NB; ++n) blocks[n].start(a, r0, kShared, h, q0 + 16 * (NB * set + n));
   if (readable) {
     for (int T0 = t0; T0 < t1; T0 += kShareTile) {
       __syncthreads();
@@ -762,7 +760,7 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const i32x4 r0,
       for (int row = first; row < first + tokens; row += STEP) {
         const int from = T0 + row;
         if (from >= t1) break;
-        attend_step<T, FP8, D, SUB, NB>(a, blocks, from, from + STEP > least, lds_k + row * S::KC, lds_v + row * S::KC, scales + row);
+        attend_step<T, FP8, D, SUB, NB>(a, blocks, t1 - from, lds_k + row * S::KC, lds_v + row * S::KC, scales + row);
       }
     }
   }
@@ -812,7 +810,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 6
   // The first 2 * shared_blocks workgroups take shared and other items in turn, the rest other items: what runs at the same
   // time on a CU is some of each (shared parts are bound by arithmetic, the others by memory).  A turn is one workgroup for
   // every CU: consecutive workgroups go to the XCDs, their shader engines and CUs in turn, so that a shorter period would
-  // give all shared items to some of them (turns of 8 workgroups: shared parts alone took 99 us, now XXX).  The grid fills the
+  // give all shared items to some of them (32 x 16 rows, 5500 shared tokens: turns of 8 workgroups 108 us in e4m3 and 115 in bf16, of 256 74 and 85).  The grid fills the
   // chip about once and strides over the items: a workgroup without work costs its slot a microsecond or two.
   int block = blockIdx.x;
   if (block < 2 * a.shared_blocks && block % (2 * kTurn) < kTurn) {
@@ -937,6 +935,7 @@ int lfm2_shared_attention(void* out, const void* q, const void* k_cache, const v
   LFM2_REQUIRE(!block_table || (page > 0 && max_blocks > 0 && max_blocks * (int64_t)page >= capacity), "shared_attention: bad page geometry");
   const int align = kv_fp8 ? (D > 16 ? D : 16) : 8;
   LFM2_REQUIRE(c0 % align == 0 && c1 % align == 0 && c2 % align == 0, "shared_attention: cache strides must be multiples of %d elements", align);
+  LFM2_REQUIRE(c1 >= 0 && c1 < (1 << 23), "shared_attention: tokens of the cache are more than 2^23 elements apart");   // 128 rows in 31 bits
   SharedArgs a;
   a.out = out; a.q = q; a.kc = k_cache; a.vc = v_cache; a.ks = k_scales; a.vs = v_scales;
   a.schedule = schedule; a.table = block_table;

@@ -634,7 +634,10 @@ def attend_shared(q, k_cache, v_cache, k_scales, v_scales, positions, prefix: Sh
     _call_on(device, "lfm2_shared_attention", out, q, k_cache, v_cache, k_scales, v_scales, schedule, block_table,
              0 if block_table is None else block_table.size(1), int(page), ws, rows, query_heads, heads, dim, capacity, pools, *strides,
              float(scale if scale is not None else dim ** -0.5), int(fp8), _code(q.dtype))
-    return quantize_rows(out.view(rows, query_heads * dim)) if quantized else out
+    if not quantized:
+        return out
+    with torch.cuda.device(device):
+        return quantize_rows(out.view(rows, query_heads * dim))
 
 
 def prefill_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float | None = None):

@@ -320,3 +320,32 @@ def test_value_scales_of_any_size(ops):
     batch.vs[:, 3] = 0.0
     batch.dvs.copy_(batch.vs.to(DEV))
     batch.check(ops)
+
+
+@pytest.mark.parametrize("fp8", (False, True))
+@pytest.mark.parametrize("page", (0, 16))
+def test_rows_that_end_inside_the_prefix_do_not_meet_what_is_behind_their_end(ops, fp8, page):
+    """The other rows of the group see infinities and NaN there, as they must; a row that ends before them does not."""
+    own = (3, -60, -99, 40, -1, 0, 5, 7, 8)
+    batch = Batch([(6, 100, 0), (3, 130, 0)], own, fp8=fp8, page=page, seed=22)
+    want, bound = batch.expected()
+    lead = batch.map[batch.leader[0]]
+    short = [b for b in range(6) if batch.lens[b] < 100]
+    assert len(short) == 3
+    for host, device in ((batch.v, batch.dv), (batch.vs, batch.dvs) if fp8 else (batch.k, batch.dk)):
+        at = int(batch.table[batch.leader[0], 99 // 16]) if page else lead
+        device.view(torch.uint8 if host.element_size() == 1 else host.dtype)[at, 99 % 16 if page else 99] = 0x7f if host.element_size() == 1 else math.inf
+    got = batch.run(ops).double().cpu()
+    for b in range(batch.rows):
+        if b >= 6 or b in short:
+            assert ((got[b] - want[b]).abs() <= bound[b]).all(), b
+        else:
+            assert not torch.isfinite(got[b]).all(), b
+
+
+def test_refuses_tokens_too_far_apart(ops):
+    storage = torch.zeros((1 << 23) + 64, dtype=torch.bfloat16, device=DEV)
+    cache = storage.as_strided((1, 2, 1, 64), ((1 << 23) + 64, 1 << 23, 64, 1))
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="apart"):
+        ops.attend_shared(torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device=DEV), cache, cache, None, None, ints(0), ops.SharedPrefix(ints(0, 1), ints(0), ints(1)))
