@@ -45,6 +45,17 @@ class LFM25HybridCache:
         return LFM25HybridCache(cut(self.k_cache), cut(self.v_cache), cut(self.conv_state), self.seq_lens[start:end],
                                 cut(self.k_scales), cut(self.v_scales))
 
+    def every(self, step: int) -> "LFM25HybridCache":
+        """Slots 0, step, 2 step ..."""
+        cut = lambda t: None if t is None else t[:, ::step]
+        return LFM25HybridCache(cut(self.k_cache), cut(self.v_cache), cut(self.conv_state), self.seq_lens[::step],
+                                cut(self.k_scales), cut(self.v_scales))
+
+    def spread_state(self, step: int) -> None:
+        """Conv state and length of every step-th slot to the step - 1 slots behind it (keys and values stay where they are)."""
+        self.conv_state.copy_(self.conv_state[:, ::step].repeat_interleave(step, dim=1))
+        self.seq_lens.copy_(self.seq_lens[::step].repeat_interleave(step))
+
     @property
     def max_slots(self) -> int:
         return int(self.seq_lens.numel())

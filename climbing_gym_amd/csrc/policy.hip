@@ -129,7 +129,9 @@ struct LogprobArgs {
   float temperature;
 };
 
-// One workgroup per row; reads the row once.  stats[row] = (max, log s, entropy, 0) for the gradient.
+// One workgroup per row; reads the row once.  stats[row] = (max, log s, entropy, 0) for the gradient.  Bound by reading:
+// 4096 rows of 65536 bf16 values (537 MB) take 77 us, 7.0 TB/s, as fast as this card reads anything; a call of a few rows is
+// the latency of one (6.5 us).
 template <typename T, int THREADS, bool ENTROPY, bool STREAM>
 __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) {
   __shared__ float scratch[THREADS / 64];
@@ -211,12 +213,13 @@ struct BackwardArgs {
 };
 constexpr int kBackwardVecs = 4;   // 16-byte pieces per thread
 
-// Elementwise given the row's statistics: workgroup (x, row) covers 256 * kBackwardVecs pieces of a row.
+// Elementwise given the row's statistics: workgroup (x, row) covers 256 * kBackwardVecs pieces of a row.  Bound by reading
+// and writing: 4096 rows of 65536 bf16 values (1.07 GB) take 188 us, 5.7 TB/s (a copy on this card: 4.7).
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(BackwardArgs a) {
   constexpr int VE = RowVec<T>::N;
   typedef typename RowVec<T>::type vec;
-  const int64_t row = blockIdx.y + (int64_t)blockIdx.z * gridDim.y, target = a.targets[row];
+  const int64_t row = blockIdx.y, target = a.targets[row];
   const int64_t nvec = a.V / VE, first = (int64_t)blockIdx.x * (256 * kBackwardVecs) + threadIdx.x;
   T* out = (T*)a.grad + row * a.grad_stride;
   const bool has_tail = blockIdx.x == 0 && threadIdx.x < a.V - nvec * VE;
@@ -377,7 +380,8 @@ template <int WAVES> __device__ __forceinline__ int block_sum_int(int v, int* sc
   return t;
 }
 
-// Tokens that count, per sequence (per block of kCountBlock tokens without sequences): one workgroup each.
+// Tokens that count, per sequence (per block of kCountBlock tokens without sequences): one workgroup each.  This and the two
+// kernels after the next are chains of dependent loads, not of bytes: 16384 tokens of 64 sequences take 5, 11 and 4 us.
 __global__ void __launch_bounds__(256) policy_count_kernel(int32_t* counts, LossArgs a) {
   __shared__ int scratch[4];
   const int64_t s = blockIdx.x;
@@ -392,7 +396,9 @@ __global__ void __launch_bounds__(256) policy_count_kernel(int32_t* counts, Loss
 // The per-token part: gradients out, sums of the terms per workgroup.  Sums are kept in 64 bits and joined in a fixed
 // order, so the result does not depend on how workgroups are scheduled.
 constexpr int kLossTerms = 6;          // policy, kl, entropy, cut, ratio, excess
-constexpr int kLossTokens = 1024;      // tokens per workgroup of 256 threads
+// Tokens per workgroup of 256 threads, each of which sweeps all sequences.  With 512 a loss of 16384 tokens (64 sequences)
+// takes 12 us instead of 14, and one of 2^20 tokens (1024 sequences) 28 instead of 21.
+constexpr int kLossTokens = 1024;
 // What a token brings, read before anything is known about its weight (a token that does not count is read and not used).
 struct TokenInputs {
   float logprob, old, ref, entropy, advantage;
@@ -513,7 +519,9 @@ policy_finish_kernel(LossArgs a, const double* partials, const int* tokens, int6
   __syncthreads();
   if (threadIdx.x == 0) store_loss(a, out, *tokens, loss, stats);
 }
-// Few tokens and sequences: one workgroup counts, weighs and sums everything; the bounds and counts are in LDS.
+// Few tokens and sequences: one workgroup counts, weighs and sums everything; the bounds and counts are in LDS.  One launch
+// instead of three: 1024 tokens of 16 sequences 8.6 us against 14.2, 4096 tokens 13.1 against 13.8 (of 2048 sequences 13.2
+// against 20.5); beyond that the one workgroup is the longer way.
 constexpr int kSingleTokens = 4096, kSingleSequences = 2048;
 __global__ void __launch_bounds__(1024) policy_single_kernel(LossArgs a, float* grad, float* grad_entropy, float* loss, float* stats) {
   constexpr int PER = kSingleTokens / 1024;
@@ -589,7 +597,11 @@ template <typename V, int N> __device__ __forceinline__ void forget_unpacked(V (
 }
 
 // One workgroup per row: statistics, the token's loss slope, and the row's gradient.  VECS > 0: the row is read once and
-// waits in registers (16 bytes each) while its statistics are joined; 0: a row too long for that is read twice.
+// waits in registers (16 bytes each) while its statistics are joined; 0: a row too long for that is read twice.  Bound by
+// reading and writing: 8958 rows of 65536 bf16 values, of which a fifth does not count (2.1 GB), take 382 us, 5.5 TB/s.
+// Whole calls (three to four launches), 4096 rows of 8192 / 32768 / 65536 values: 46 / 107 / 219 us, read twice 54 / 145 /
+// 270.  256 threads hold rows of up to 16 KiB: with 512, 4096 rows of 8192 values take 57.  1024 threads for the longest
+// rows that are held leave room for one row per CU at a time: 489 us for the 8958 rows, 406 with 512.
 template <typename T, int THREADS, int VECS, bool ENTROPY>
 __global__ void __launch_bounds__(THREADS) policy_gradient_kernel(GradientArgs a) {
   constexpr int VE = RowVec<T>::N;
@@ -718,8 +730,9 @@ int fill_loss(const char* name, LossArgs* a, const float* logprobs, const float*
 }
 
 // Logits of this size or more leave the last-level cache (256 MB) before anybody reads them again: the scoring pass then
-// loads them with the non-temporal hint; smaller ones stay there for the gradient.
-constexpr int64_t kStreamBytes = 192ll << 20;
+// loads them with the non-temporal hint; smaller ones stay there for the gradient.  Scoring and gradient of 134 / 210 MB: 68 /
+// 117 us with the hint, 66 / 109 without; of 288 / 537 MB: 158 / 276 with it, 171 / 300 without.
+constexpr int64_t kStreamBytes = 224ll << 20;
 
 int64_t count_slots(int64_t N, int64_t S, bool cu) { return cu ? S : (N + kCountBlock - 1) / kCountBlock; }
 int64_t loss_blocks(int64_t N) { return (N + kLossTokens - 1) / kLossTokens; }
@@ -764,6 +777,8 @@ int lfm2_token_logprobs(float* logprobs, float* entropy, float* stats, const voi
 #define LOGPROBS_(THREADS, ENTROPY, STREAM) \
   hipLaunchKernelGGL((token_logprobs_kernel<T, THREADS, ENTROPY, STREAM>), dim3((unsigned)N), dim3(THREADS), 0, s, a)
   DISPATCH_LOGITS(dtype, "token_logprobs",
+    // 4096 rows of 4096 / 8192 values: 7.7 / 14.5 us with 128 threads, 11.7 / 16.2 with 512; of 65536: 85 and 83; 64 rows of
+    // 16384: 5.2 and 4.2
     const bool stream_once = N * row_stride * (int64_t)sizeof(T) >= kStreamBytes;
     if (V <= 8192) {
       if (stream_once) { if (entropy) LOGPROBS_(128, true, true); else LOGPROBS_(128, false, true); }
@@ -786,7 +801,7 @@ int lfm2_token_logprobs_backward(void* grad, int64_t grad_stride, const void* lo
   LFM2_REQUIRE(temperatures || temperature > 0.f, "token_logprobs_backward: temperature must be positive");
   const BackwardArgs a{grad, logits, targets, stats, grad_logprobs, grad_entropy, temperatures, grad_stride, row_stride, V, temperature};
   hipStream_t s = (hipStream_t)stream;
-  // rows over y and z: a grid's y and z hold 65535 each; rows are split evenly, so z * y is N exactly or the launch is refused
+  // a grid's y holds 65535 rows
   DISPATCH_LOGITS(dtype, "token_logprobs_backward",
     const int64_t pieces = V / RowVec<T>::N;
     const unsigned x = (unsigned)(pieces ? (pieces + 256 * kBackwardVecs - 1) / (256 * kBackwardVecs) : 1);

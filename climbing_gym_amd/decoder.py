@@ -17,7 +17,7 @@ import torch
 from . import ops
 from .cache import LFM25HybridCache
 from .config import LFM25SamplingConfig
-from .engine import LFM25GenerationOutput
+from .engine import LFM25GenerationOutput, prefix_of_repeats
 from ._checks import reject
 
 
@@ -38,6 +38,7 @@ class _DecodeGraph:
     logits: torch.Tensor
     graph: object
     active: torch.Tensor | None = None
+    prefix: ops.SharedPrefix | None = None   # for rows whose groups share the first part of their history
     compact_graphs: dict = field(default_factory=dict)
 
 
@@ -67,13 +68,16 @@ class LFM25HIPDecoder:
     def __init__(self, engine, *, max_graphs: int = 2, max_prefill_tokens: int = 4096, finish_check_interval: int = 32,
                  skip_finished_attention: bool = True, fp8_mlp: bool = False, fp8_kv: bool = False,
                  adaptive_batching: bool = False, fp8_lm_head: bool = False, fp8_operators: bool = False,
-                 capture: bool = True):
+                 capture: bool = True, shared_prefix: bool = False):
         reject(max_graphs <= 0, "max_graphs must be > 0")
         reject(max_prefill_tokens <= 0, "max_prefill_tokens must be positive")
         reject(type(finish_check_interval) is not int or finish_check_interval <= 0,
                "finish_check_interval must be a positive integer")
+        reject(shared_prefix and adaptive_batching, "shared prefixes and adaptive batching cannot be combined: a group's rows stay together")
+        reject(shared_prefix and engine.dtype not in (torch.bfloat16, torch.float16), "shared prefixes need a bf16 or fp16 model")
         self.engine = engine
         self.max_graphs = max_graphs
+        self.shared_prefix = bool(shared_prefix)
         self.max_prefill_tokens = max_prefill_tokens
         self.finish_check_interval = finish_check_interval
         self.skip_finished_attention = bool(skip_finished_attention)
@@ -115,9 +119,9 @@ class LFM25HIPDecoder:
         self.fp8_weights.clear()
 
     # ------------------------------------------------------------------ capture
-    def _forward(self, cache, tokens, active=None, *, slot_ids=None, positions=None, logits_out=None, gather=None):
+    def _forward(self, cache, tokens, active=None, *, slot_ids=None, positions=None, logits_out=None, gather=None, prefix=None):
         return self.engine._decode_forward(cache, tokens, active, slot_ids=slot_ids, positions=positions, fp8=self.fp8_weights,
-                                           logits_out=logits_out, gather=gather)
+                                           logits_out=logits_out, gather=gather, prefix=prefix)
 
     def _capture(self, step, before_warmup=None, probe=None):
         """Two warm-up launches, then record `step` into a HIP graph on the decoder's capture stream.  `probe` is
@@ -157,9 +161,10 @@ class LFM25HIPDecoder:
         return graph
 
     @torch.inference_mode()
-    def _get_graph(self, batch_size: int, cache_len: int, *, masked: bool = False) -> _DecodeGraph:
+    def _get_graph(self, batch_size: int, cache_len: int, *, masked: bool = False, groups: int = 0) -> _DecodeGraph:
+        """`groups`: the rows are that many equal groups, each of which reads its prefix from its first row's slot."""
         capacity = graph_capacity(cache_len, batch_size, self.engine.max_model_len)
-        key = (batch_size, capacity, masked)
+        key = (batch_size, capacity, masked, groups) if groups else (batch_size, capacity, masked)
         if key in self.graphs:
             self.graphs.move_to_end(key)
             return self.graphs[key]
@@ -174,15 +179,18 @@ class LFM25HIPDecoder:
         saved = torch.zeros((batch_size, engine.config.vocab_size), device=engine.device, dtype=engine.dtype) if masked else None
         if saved is None and not self.capture:
             saved = torch.zeros((batch_size, engine.config.vocab_size), device=engine.device, dtype=engine.dtype)
+        prefix = None
+        if groups:
+            prefix = prefix_of_repeats(groups, batch_size // groups, torch.zeros(groups, device=engine.device, dtype=torch.int32))
         holder = {}
 
         def step():
             # masked steps write only the live rows of `saved`; uncaptured steps write all of it, so that one stable
             # buffer holds the logits either way
-            holder["logits"] = self._forward(cache, tokens, active, logits_out=saved)
+            holder["logits"] = self._forward(cache, tokens, active, logits_out=saved, prefix=prefix)
 
         graph = self._capture(step, before_warmup=cache.seq_lens.zero_)
-        entry = _DecodeGraph(cache, tokens, holder["logits"] if self.capture else saved, graph, active)
+        entry = _DecodeGraph(cache, tokens, holder["logits"] if self.capture else saved, graph, active, prefix=prefix)
         self.graphs[key] = entry
         if batch_size >= 64:
             torch.cuda.empty_cache()
@@ -206,7 +214,7 @@ class LFM25HIPDecoder:
             cache.conv_state.copy_(conv_state)
 
         def step():
-            self._forward(cache, entry.input_tokens, entry.active, logits_out=logits)
+            self._forward(cache, entry.input_tokens, entry.active, logits_out=logits, prefix=entry.prefix)
 
         graph = self._capture(step, before_warmup=restore, probe=probe)
         return graph
@@ -260,15 +268,26 @@ class LFM25HIPDecoder:
         batch = prompts * repeats
         k = sampling.behavior_topk
         reject(k > vocab, 'Behavior head exceeds the vocabulary')
-        entry = self._get_graph(batch, cache_len, masked=self.adaptive_batching) if new_tokens > 1 else None
-        direct = entry is not None and repeats == 1
+        # Repeats that share their prompt's history: it is prefilled into the first repeat's slot and stays there.  Finished
+        # rows then sit out steps (a masked graph): shortening them, as below, would append to that slot's beginning.
+        sharing = self.shared_prefix and repeats > 1 and new_tokens > 1
+        reject(sharing and batch > ops.MAX_SHARED_ROWS, f"more than {ops.MAX_SHARED_ROWS} rows share prefixes")
+        entry = (self._get_graph(batch, cache_len, masked=self.adaptive_batching or sharing, groups=prompts if sharing else 0)
+                 if new_tokens > 1 else None)
+        direct = entry is not None and (repeats == 1 or sharing)
         prefix = engine.prefill(input_ids, cu_seqlens, max_seqlen, max_cache_len=max_seqlen,
                                 cache=entry.cache if direct else None, max_prefill_tokens=self.max_prefill_tokens,
-                                logits_buffer=entry.logits if direct else None)
+                                logits_buffer=entry.logits if direct else None,
+                                slots=range(0, batch, repeats) if sharing else None)
         if entry is not None and not direct:
             rows = torch.arange(prefix.batch_size, device=device).repeat_interleave(repeats)
             entry.cache.copy_prefix_from(prefix.cache, rows, max_seqlen)
-        logits = prefix.next_token_logits if repeats == 1 else prefix.next_token_logits.repeat_interleave(repeats, dim=0)
+        if sharing:
+            entry.cache.spread_state(repeats)
+            entry.prefix.lengths.copy_(prefix.prompt_lengths)
+            logits = prefix.next_token_logits[::repeats].repeat_interleave(repeats, dim=0)
+        else:
+            logits = prefix.next_token_logits if repeats == 1 else prefix.next_token_logits.repeat_interleave(repeats, dim=0)
         seen = engine._build_seen_token_mask(prefix, repeats, sampling)
         del prefix
 

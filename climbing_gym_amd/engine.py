@@ -49,6 +49,7 @@ class LFM25DecodeBatch:
     prompt_indices: torch.Tensor
     repeat_indices: torch.Tensor
     alive: torch.Tensor
+    prefix: ops.SharedPrefix | None = None   # of all slots, when the repeats of a prompt share one copy of its history
 
     @property
     def batch_size(self) -> int:
@@ -63,6 +64,15 @@ class LFM25StepOutput:
     finished: torch.Tensor
     finish_reasons: torch.Tensor
     logits: torch.Tensor
+
+
+@dataclass(frozen=True)
+class LFM25PolicyObjective:
+    """`ops.policy_loss_forward` of given completions under the engine's weights: the loss, its statistics (policy term,
+    KL, entropy, share of ratios cut, mean ratio, mean of r - 1 - log r, tokens) and every token's log-probability."""
+    loss: float
+    stats: tuple
+    logprobs: list
 
 
 @dataclass(frozen=True)
@@ -144,6 +154,12 @@ def flatten_token_batches(input_ids: Sequence[Sequence[int]], *, device=None):
     return flat, cu_host.to(device), max(lengths)
 
 
+def prefix_of_repeats(prompts: int, repeats: int, prompt_lengths: torch.Tensor) -> ops.SharedPrefix:
+    """Rows i * repeats .. (i + 1) * repeats - 1 share prompt i, which the first of them holds."""
+    bounds = torch.arange(0, prompts * repeats + 1, repeats, device=prompt_lengths.device, dtype=torch.int32)
+    return ops.SharedPrefix(bounds, bounds[:-1].clone(), prompt_lengths.to(torch.int32).clone())
+
+
 class LFM25Engine:
     def __init__(self, weights: LFM25PackedWeights, *, max_model_len: int | None = None) -> None:
         reject(weights.device.type != "cuda", "this engine runs on the GPU only; weights must live on a HIP device")
@@ -203,16 +219,20 @@ class LFM25Engine:
 
     def enable_cuda_graphs(self, *, max_graphs: int = 2, bf16_weight_packing: bool = True, max_prefill_tokens: int = 4096,
                            fp8_mlp: bool = False, fp8_kv: bool = False, adaptive_batching: bool = False,
-                           fp8_lm_head: bool = False, fp8_operators: bool = False, capture: bool = True) -> None:
+                           fp8_lm_head: bool = False, fp8_operators: bool = False, capture: bool = True,
+                           shared_prefix: bool = False) -> None:
         """Same switch as the reference (lfm25_engine.py:980-997); graphs are HIP graphs.  `fp8_operators` extends
-        W8A8 to the QKV/out and conv in/out projections; `bf16_weight_packing` is accepted and ignored."""
+        W8A8 to the QKV/out and conv in/out projections; `bf16_weight_packing` is accepted and ignored.  With
+        `shared_prefix`, `generate` with repeats keeps one copy of a prompt's keys and values and reads it once per step for
+        all its completions."""
         from .decoder import LFM25HIPDecoder
         reject(self._decoder_busy, "Close the native generation session before reconfiguring CUDA graphs", RuntimeError)
         if self._cuda_decoder is not None:
             self._cuda_decoder.clear()
         self._cuda_decoder = LFM25HIPDecoder(self, max_graphs=max_graphs, max_prefill_tokens=max_prefill_tokens,
                                              fp8_mlp=fp8_mlp, fp8_kv=fp8_kv, adaptive_batching=adaptive_batching,
-                                             fp8_lm_head=fp8_lm_head, fp8_operators=fp8_operators, capture=capture)
+                                             fp8_lm_head=fp8_lm_head, fp8_operators=fp8_operators, capture=capture,
+                                             shared_prefix=shared_prefix)
 
     enable_hip_graphs = enable_cuda_graphs
 
@@ -353,11 +373,12 @@ class LFM25Engine:
 
     # ------------------------------------------------------------------ decode step (one token per row)
     def _decode_forward(self, cache: LFM25HybridCache, tokens, active=None, *, slot_ids=None, positions=None, fp8=None,
-                        logits_out=None, gather=None):
+                        logits_out=None, gather=None, prefix: ops.SharedPrefix | None = None):
         """One token for every row (lfm25_cuda.py:128-192).  Rows index cache slots directly, or through `slot_ids`
         (then `positions` are the rows' lengths and -1 marks padding).  With `logits_out` ([slots, vocab]) the head
         projection writes the live rows' logits there (row -> its slot) and the other rows keep theirs: the
-        `_scatter_logits` step of lfm25_batching.py:99-101 without a copy."""
+        `_scatter_logits` step of lfm25_batching.py:99-101 without a copy.  With `prefix`, rows of a group read the first
+        part of their history from one slot."""
         cfg = self.config
         fp8 = self._fp8() if fp8 is None else fp8
         rows = tokens.numel()
@@ -373,8 +394,11 @@ class LFM25Engine:
             positions, schedule = ops.decode_begin(cache.seq_lens, capacity=cache.max_seq_len,
                                                    gather=(gather[0], gather[1], slot_ids, tokens, positions, active))
         else:
-            schedule = ops.decode_schedule(positions, active, slot_ids, capacity=cache.max_seq_len)
+            schedule = None if prefix is not None else ops.decode_schedule(positions, active, slot_ids, capacity=cache.max_seq_len)
             advance_after = True
+        if prefix is not None:
+            schedule = ops.shared_schedule(positions, prefix, active, slot_ids, capacity=cache.max_seq_len,
+                                           query_heads=cfg.num_attention_heads, kv_heads=cfg.num_key_value_heads, head_dim=cfg.head_dim)
 
         probe = self._step_probe
 
@@ -382,8 +406,12 @@ class LFM25Engine:
             # `probe(kind, index, phase)`, when a measurement asks for it, brackets the call on the launch stream
             if probe is not None:
                 probe("attention", i, 0)
-            out = ops.attend(q, cache.k_cache[i], cache.v_cache[i], k_scales, v_scales, positions, active=active,
-                             scale=self._scaling, slot_ids=slot_ids, schedule=schedule, quantized=quantized)
+            if prefix is None:
+                out = ops.attend(q, cache.k_cache[i], cache.v_cache[i], k_scales, v_scales, positions, active=active,
+                                 scale=self._scaling, slot_ids=slot_ids, schedule=schedule, quantized=quantized)
+            else:
+                out = ops.attend_shared(q, cache.k_cache[i], cache.v_cache[i], k_scales, v_scales, positions, prefix, active=active,
+                                        scale=self._scaling, slot_ids=slot_ids, schedule=schedule, quantized=quantized)
             if probe is not None:
                 probe("attention", i, 1)
             return out
@@ -552,20 +580,31 @@ class LFM25Engine:
 
     # ------------------------------------------------------------------ fork / decode_step
     @torch.inference_mode()
-    def fork(self, prefix: LFM25PrefixBatch, repeats: int, *, max_cache_len: int | None = None) -> LFM25DecodeBatch:
+    def fork(self, prefix: LFM25PrefixBatch, repeats: int, *, max_cache_len: int | None = None,
+             share_prefix: bool = False) -> LFM25DecodeBatch:
+        """Every prompt `repeats` times (lfm25_engine.py:761).  With `share_prefix` only the first repeat of a prompt gets
+        its keys and values; the others read them there (`ops.attend_shared`), once for all of them per step."""
         reject(repeats <= 0, "repeats must be > 0")
+        reject(share_prefix and self.dtype not in (torch.bfloat16, torch.float16), "shared prefixes need a bf16 or fp16 model")
         prompts = prefix.batch_size
         total = prompts * int(repeats)
         cache_len = int(max_cache_len or prefix.cache.max_seq_len)
         reject(cache_len < prefix.cache.max_seq_len, "max_cache_len cannot be smaller than the prefix cache")
         cache = self._empty_cache(max_slots=total, max_seq_len=cache_len)
         arange = lambda n: torch.arange(n, device=self.device, dtype=torch.long)
-        cache.copy_prefix_from(prefix.cache, arange(prompts).repeat_interleave(repeats), prefix.cache.max_seq_len)
-        return LFM25DecodeBatch(cache, arange(total), arange(prompts).repeat_interleave(repeats),
-                                arange(repeats).repeat(prompts), torch.ones(total, device=self.device, dtype=torch.bool))
+        prompt_of = arange(prompts).repeat_interleave(repeats)
+        shared = None
+        if share_prefix:
+            cache.every(int(repeats)).copy_prefix_from(prefix.cache, arange(prompts), prefix.cache.max_seq_len)
+            cache.spread_state(int(repeats))
+            shared = prefix_of_repeats(prompts, int(repeats), prefix.prompt_lengths)
+        else:
+            cache.copy_prefix_from(prefix.cache, prompt_of, prefix.cache.max_seq_len)
+        return LFM25DecodeBatch(cache, arange(total), prompt_of, arange(repeats).repeat(prompts),
+                                torch.ones(total, device=self.device, dtype=torch.bool), shared)
 
     @torch.inference_mode()
-    def _append_decode_tokens(self, cache: LFM25HybridCache, slot_ids, input_tokens):
+    def _append_decode_tokens(self, cache: LFM25HybridCache, slot_ids, input_tokens, prefix: ops.SharedPrefix | None = None):
         """Eager decode of one token for the given slots with the reference's capacity checks
         (lfm25_engine.py:1232-1243)."""
         slot_ids = slot_ids.to(device=self.device, dtype=torch.long).reshape(-1)
@@ -577,14 +616,18 @@ class LFM25Engine:
         reject(torch.any(positions >= cache.max_seq_len), "cache capacity exceeded", RuntimeError)
         reject(torch.any(positions >= self.max_model_len), "position exceeds engine max_model_len", RuntimeError)
         active = torch.ones(slot_ids.numel(), device=self.device, dtype=torch.bool)
-        return self._decode_forward(cache, input_tokens, active, slot_ids=slot_ids.to(torch.int32), positions=positions.contiguous())
+        if prefix is not None:   # groups of all slots -> groups of the rows that take part
+            reject(torch.any(slot_ids[1:] < slot_ids[:-1]), "slots that share prefixes must be in ascending order")
+            prefix = ops.SharedPrefix(torch.searchsorted(slot_ids, prefix.starts.long()).to(torch.int32), prefix.slots, prefix.lengths)
+        return self._decode_forward(cache, input_tokens, active, slot_ids=slot_ids.to(torch.int32), positions=positions.contiguous(),
+                                    prefix=prefix)
 
     @torch.inference_mode()
     def decode_step(self, state: LFM25DecodeBatch, input_tokens, sampling: LFM25SamplingConfig | None = None) -> LFM25StepOutput:
         sampling = sampling or LFM25SamplingConfig()
         input_tokens = input_tokens.to(device=self.device, dtype=torch.long).reshape(-1)
         reject(input_tokens.numel() != state.active_slot_ids.numel(), "input_tokens must have one token per active slot")
-        logits = self._append_decode_tokens(state.cache, state.active_slot_ids, input_tokens)
+        logits = self._append_decode_tokens(state.cache, state.active_slot_ids, input_tokens, state.prefix)
         tokens, raw, tempered = self._sample(logits, sampling, step=0, sampling_logprobs=sampling.return_logprobs)
         reasons = self._finish_reasons(tokens, sampling)
         keep = sampling.return_logprobs
@@ -638,14 +681,29 @@ class LFM25Engine:
     @torch.inference_mode()
     def score_completions(self, prompts, completions, *, max_prefill_tokens: int = 4096, head_chunk_size: int = 256):
         """Raw log-probabilities of given completions through the packed prefill kernels (lfm25_engine.py:1108-1163)."""
+        result = [()] * len(prompts)
+        for group, selected, target in self._completion_rows(prompts, completions, max_prefill_tokens, head_chunk_size):
+            scores = []
+            for off in range(0, target.numel(), head_chunk_size):
+                logits = self._linear(selected[off:off + head_chunk_size].contiguous(), self.weights.lm_head_weight, {}).float()
+                pick = target[off:off + head_chunk_size]
+                scores.append(logits.gather(1, pick[:, None])[:, 0] - torch.logsumexp(logits, -1))
+            flat, cursor = torch.cat(scores).cpu().tolist(), 0
+            for i in group:
+                result[i] = tuple(flat[cursor:cursor + len(completions[i])])
+                cursor += len(completions[i])
+        return result
+
+    def _completion_rows(self, prompts, completions, max_prefill_tokens: int, head_chunk_size: int):
+        """For each packed chunk of sequences: their indices, the final-norm hidden states that predict their completion
+        tokens, and those tokens."""
         reject(len(prompts) != len(completions), 'prompts and completions must have equal lengths')
         reject(max_prefill_tokens <= 0 or head_chunk_size <= 0, 'scoring chunk sizes must be positive')
         reject(any(not p or not c for p, c in zip(prompts, completions)),
                'scoring requires nonempty prompts and completions')
         sequences = [list(p) + list(c) for p, c in zip(prompts, completions)]
         reject(any(len(s) > self.max_model_len for s in sequences), 'scored sequence exceeds max_model_len')
-        cfg, fp8 = self.config, self._fp8()
-        result = [()] * len(sequences)
+        fp8 = self._fp8()
         order = sorted(range(len(sequences)), key=lambda i: len(sequences[i]))
         lengths = [len(sequences[i]) for i in order]
         for start, end in plan_packed_chunks(lengths, min(int(max_prefill_tokens), MAX_PACKED_TOKENS)):
@@ -659,17 +717,45 @@ class LFM25Engine:
                 targets.extend(completions[i])
                 base += len(sequences[i])
             selected = hidden.index_select(0, torch.tensor(rows, device=self.device))
-            target = torch.tensor(targets, device=self.device, dtype=torch.long)
-            scores = []
+            yield group, selected, torch.tensor(targets, device=self.device, dtype=torch.long)
+
+    @torch.inference_mode()
+    def policy_objective(self, prompts, completions, old_logprobs, advantages, *, ref_logprobs=None, temperature: float = 1.0,
+                         config: ops.PolicyLossConfig = ops.PolicyLossConfig(), max_prefill_tokens: int = 4096,
+                         head_chunk_size: int = 1024) -> LFM25PolicyObjective:
+        """The clipped policy loss of sampled completions under the weights the engine holds now, for instance after
+        `sync_from_model`: how far the policy has moved from the one that drew them.  `old_logprobs` (and `ref_logprobs`):
+        per completion, one value per token, at the sampling temperature; `advantages`: one number per completion, or one
+        per token like these."""
+        lengths = [len(c) for c in completions]
+        reject(not lengths, 'an objective needs at least one completion')
+        per_sequence = len(advantages) > 0 and not hasattr(advantages[0], '__len__')
+        flat = {}
+        for name, values, wanted in (('old_logprobs', old_logprobs, lengths), ('ref_logprobs', ref_logprobs, lengths),
+                                     ('advantages', advantages, None if per_sequence else lengths)):
+            if values is None:
+                continue
+            reject(len(values) != len(lengths) or (wanted is not None and [len(v) for v in values] != wanted),
+                   f'{name} must match the completions')
+            numbers = [float(x) for x in values] if wanted is None else [float(x) for v in values for x in v]
+            flat[name] = torch.tensor(numbers, dtype=torch.float32).to(self.device)
+        bounds = [0, *itertools.accumulate(lengths)]
+        logprobs = torch.empty(bounds[-1], device=self.device, dtype=torch.float32)
+        entropy = torch.empty_like(logprobs) if config.entropy_coef != 0.0 else None
+        for group, selected, target in self._completion_rows(prompts, completions, max_prefill_tokens, head_chunk_size):
+            place = torch.tensor([t for i in group for t in range(bounds[i], bounds[i + 1])], device=self.device)
             for off in range(0, target.numel(), head_chunk_size):
-                logits = self._linear(selected[off:off + head_chunk_size].contiguous(), self.weights.lm_head_weight, {}).float()
-                pick = target[off:off + head_chunk_size]
-                scores.append(logits.gather(1, pick[:, None])[:, 0] - torch.logsumexp(logits, -1))
-            flat, cursor = torch.cat(scores).cpu().tolist(), 0
-            for i in group:
-                result[i] = tuple(flat[cursor:cursor + len(completions[i])])
-                cursor += len(completions[i])
-        return result
+                part = slice(off, off + head_chunk_size)
+                logits = self._linear(selected[part].contiguous(), self.weights.lm_head_weight, {})
+                scores, spread, _ = ops.token_logprobs_forward(logits, target[part], temperature=temperature, entropy=entropy is not None)
+                logprobs[place[part]] = scores
+                if entropy is not None:
+                    entropy[place[part]] = spread
+        loss, stats, _, _ = ops.policy_loss_forward(
+            logprobs, flat['old_logprobs'], flat['advantages'], ref_logprobs=flat.get('ref_logprobs'), entropy=entropy,
+            cu_seqlens=torch.tensor(bounds, dtype=torch.int32).to(self.device), per_sequence=per_sequence, config=config)
+        values = logprobs.cpu().tolist()
+        return LFM25PolicyObjective(float(loss), tuple(stats.cpu().tolist()), [tuple(values[a:b]) for a, b in zip(bounds, bounds[1:])])
 
     def _prefill_hidden(self, cache, tokens, lengths, fp8):
         """Final-norm hidden states of every packed token (the `return_hidden` form of lfm25_engine.py:1097-1098)."""

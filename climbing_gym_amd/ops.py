@@ -548,6 +548,9 @@ def decode(q, k, v, k_cache, v_cache, k_scales, v_scales, positions, *, active=N
                   window=window, schedule=schedule)
 
 
+MAX_SHARED_ROWS = 4096   # rows, and groups, a work list of `shared_schedule` holds
+
+
 @dataclass(frozen=True)
 class SharedPrefix:
     """Rows of a decode batch in groups that share the first part of their history (the completions of one prompt): group g
@@ -840,6 +843,8 @@ def _gradient_output(out, logits):
     same = out.data_ptr() == logits.data_ptr() and _row_stride(out) == _row_stride(logits)
     reject(not same and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr(),
            "out must be the logits themselves or share no storage with them")
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)   # a graph that saved it must not run on what is written here
     return out
 
 
@@ -1029,8 +1034,8 @@ def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: 
 def policy_gradient(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, *,
                     mask=None, ref_logprobs=None, cu_seqlens=None, per_sequence: bool = False, temperature=1.0,
                     config: PolicyLossConfig = PolicyLossConfig(), grad_scale: float = 1.0, out: torch.Tensor | None = None):
-    """`token_logprobs`, `policy_loss` and the gradient of the logits in one pass over the rows that count, without the
-    second reading of the logits that a backward call makes: returns (loss, stats, log-probabilities fp32 [N],
+    """`token_logprobs`, `policy_loss` and the gradient of the logits in one call, without the second reading of the logits that
+    a backward call makes (rows of up to 128 KiB are read once): returns (loss, stats, log-probabilities fp32 [N],
     grad_scale * d loss / d logits in the logits' dtype).  Arguments as in those two functions; a token counts when `mask`
     says so and its target is not negative; rows that do not count get zeros.  For `logits.backward(gradient)` of the
     caller's own graph.  `out` (where the gradient goes) may be the logits."""
