@@ -121,14 +121,7 @@ def load():
     return lib
 
 
-def _arg(value):
-    if value is None:
-        return None
-    if isinstance(value, torch.Tensor):
-        return value.data_ptr()
-    return value
-
-
+_Tensor = torch.Tensor
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _raw_device = getattr(torch._C, "_cuda_getDevice", None)
 
@@ -144,8 +137,9 @@ def stream_handle() -> int:
 
 def call(name: str, *args):
     """Invoke an int-returning entry point on the current stream (appended as the last argument)."""
-    lib = load()
-    status = getattr(lib, name)(*[_arg(a) for a in args], stream_handle())
+    lib = _lib or load()
+    # (converted in place: two dozen calls of a helper are microseconds of a small operator's call)
+    status = getattr(lib, name)(*[a.data_ptr() if isinstance(a, _Tensor) else a for a in args], stream_handle())
     if status != 0:
         message = lib.lfm2_last_error().decode()
         if status == -1:

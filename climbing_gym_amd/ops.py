@@ -42,13 +42,16 @@ def _check(*tensors):
 
 def _one_device(*tensors):
     """The device all given tensors (None: left out) live on; the launch goes to that device's current stream."""
-    device = None
+    device = index = None
     for t in tensors:
         if t is None:
             continue
-        reject(not t.is_cuda, "HIP kernels require GPU tensors")
-        reject(device is not None and t.device != device, "all tensors of a call live on one device")
-        device = t.device
+        if not t.is_cuda:
+            raise ValueError("HIP kernels require GPU tensors")
+        if device is None:
+            device, index = t.device, t.get_device()
+        elif t.get_device() != index:
+            raise ValueError("all tensors of a call live on one device")
     return device
 
 
@@ -562,7 +565,8 @@ class SharedPrefix:
 
     def check(self):
         for name, t in (("starts", self.starts), ("slots", self.slots), ("lengths", self.lengths)):
-            reject(t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous(), f"prefix {name} must be a contiguous int32 vector")
+            if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous():
+                raise ValueError(f"prefix {name} must be a contiguous int32 vector")
         reject(self.slots.numel() == 0 or self.starts.numel() != self.slots.numel() + 1 or self.lengths.numel() != self.slots.numel(),
                "a shared prefix needs one slot and one length per group and one bound more")
 
@@ -587,7 +591,7 @@ def shared_schedule(positions, prefix: SharedPrefix, active=None, slot_ids=None,
     device = _one_device(positions, prefix.starts, prefix.slots, prefix.lengths, active, slot_ids)
     reject(query_heads <= 0 or kv_heads <= 0 or query_heads % kv_heads, "query heads must be a multiple of the KV heads")
     size = _size("lfm2_shared_schedule_size", rows, int(capacity), query_heads, kv_heads, head_dim)
-    schedule = torch.empty(max(size, 4), device=device, dtype=torch.int32)
+    schedule = positions.new_empty(max(size, 4))
     _call_on(device, "lfm2_shared_schedule", schedule, positions, active, slot_ids, prefix.starts, prefix.slots, prefix.lengths,
              rows, prefix.slots.numel(), int(capacity), query_heads, kv_heads, head_dim)
     return schedule
@@ -632,7 +636,7 @@ def attend_shared(q, k_cache, v_cache, k_scales, v_scales, positions, prefix: Sh
         reject(schedule.dtype != torch.int32 or not schedule.is_contiguous()
                or schedule.numel() < _size("lfm2_shared_schedule_size", rows, capacity, query_heads, heads, dim),
                "schedule must come from shared_schedule for this batch")
-    ws = torch.empty(_size("lfm2_shared_attention_workspace", rows, capacity, query_heads, heads, dim), device=device, dtype=torch.float32)
+    ws = q.new_empty(_size("lfm2_shared_attention_workspace", rows, capacity, query_heads, heads, dim), dtype=torch.float32)
     out = torch.empty_like(q)
     _call_on(device, "lfm2_shared_attention", out, q, k_cache, v_cache, k_scales, v_scales, schedule, block_table,
              0 if block_table is None else block_table.size(1), int(page), ws, rows, query_heads, heads, dim, capacity, pools, *strides,
@@ -825,8 +829,8 @@ def _check_logits(logits, targets, temperature):
 
 
 def _check_row_values(tensor, rows: int, dtype, name: str) -> None:
-    reject(not isinstance(tensor, torch.Tensor) or tensor.dtype != dtype or tensor.shape != (rows,) or not tensor.is_contiguous(),
-           f"{name} must be a contiguous {dtype} tensor of {rows} entries")
+    if not isinstance(tensor, torch.Tensor) or tensor.dtype != dtype or tensor.shape != (rows,) or not tensor.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {rows} entries")
 
 
 def _row_stride(matrix) -> int:
@@ -836,7 +840,7 @@ def _row_stride(matrix) -> int:
 def _gradient_output(out, logits):
     """The tensor a gradient of the logits goes to: fresh, or `out` (the logits themselves, or memory apart from them)."""
     if out is None:
-        return torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+        return logits.new_empty(logits.shape)
     reject(out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device
            or (out.size(1) > 1 and out.stride(1) != 1) or (out.size(0) > 1 and out.stride(0) < out.size(1)),
            "out must match the logits in shape, dtype and device, with consecutive columns and rows that do not overlap")
@@ -856,9 +860,9 @@ def token_logprobs_forward(logits: torch.Tensor, targets: torch.Tensor, *, tempe
     (rows with a temperature <= 0 are scored at 1).  Rows of -inf only give -inf and entropy 0."""
     temperatures, value = _check_logits(logits, targets, temperature)
     device, rows = _one_device(logits, targets, temperatures), logits.size(0)
-    logprobs = torch.empty(rows, device=device, dtype=torch.float32)
-    entropies = torch.empty(rows, device=device, dtype=torch.float32) if entropy else None
-    stats = torch.empty((rows, 4), device=device, dtype=torch.float32)
+    logprobs = logits.new_empty(rows, dtype=torch.float32)
+    entropies = logprobs.new_empty(rows) if entropy else None
+    stats = logprobs.new_empty((rows, 4))
     if rows:
         _call_on(device, "lfm2_token_logprobs", logprobs, entropies, stats, logits, _row_stride(logits), targets, temperatures,
                  value, rows, logits.size(1), _code(logits.dtype))
@@ -963,9 +967,8 @@ def _check_tokens(tokens: int, old_logprobs, advantages, mask, ref_logprobs, cu_
     if ref_logprobs is not None:
         _check_row_values(ref_logprobs, tokens, torch.float32, "ref_logprobs")
     reject(config.kl_coef != 0.0 and ref_logprobs is None, "a KL term needs ref_logprobs")
-    if mask is not None:
-        reject(mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (tokens,) or not mask.is_contiguous(),
-               f"mask must be a contiguous bool tensor of {tokens} entries")
+    if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (tokens,) or not mask.is_contiguous()):
+        raise ValueError(f"mask must be a contiguous bool tensor of {tokens} entries")
     sequences = 1
     if cu_seqlens is not None:
         reject(cu_seqlens.dtype != torch.int32 or cu_seqlens.ndim != 1 or cu_seqlens.numel() < 2 or not cu_seqlens.is_contiguous(),
@@ -993,10 +996,10 @@ def policy_loss_forward(logprobs: torch.Tensor, old_logprobs: torch.Tensor, adva
         _check_row_values(entropy, tokens, torch.float32, "entropy")
     reject(config.entropy_coef != 0.0 and entropy is None, "an entropy bonus needs the tokens' entropies")
     device = _one_device(logprobs, old_logprobs, advantages, mask, ref_logprobs, entropy, cu_seqlens)
-    fresh = lambda *shape: torch.empty(shape, device=device, dtype=torch.float32)
+    fresh = old_logprobs.new_empty
     if tokens == 0:
         return (torch.zeros((), device=device), torch.zeros(7, device=device), fresh(0), None if entropy is None else fresh(0))
-    loss, stats, grad = fresh(), fresh(7), fresh(tokens)
+    loss, stats, grad = fresh(()), fresh(7), fresh(tokens)
     grad_entropy = None if entropy is None else fresh(tokens)
     workspace = fresh(_size("lfm2_policy_workspace", tokens, sequences, int(cu_seqlens is not None)))
     _call_on(device, "lfm2_policy_loss", loss, stats, grad, grad_entropy, logprobs, old_logprobs, advantages, ref_logprobs, entropy,
@@ -1045,10 +1048,10 @@ def policy_gradient(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: t
     reject(not -float("inf") < float(grad_scale) < float("inf"), "grad_scale must be finite")
     device = _one_device(logits, targets, temperatures, old_logprobs, advantages, mask, ref_logprobs, cu_seqlens)
     grad = _gradient_output(out, logits)
-    fresh = lambda *shape: torch.empty(shape, device=device, dtype=torch.float32)
+    fresh = old_logprobs.new_empty
     if tokens == 0:
         return torch.zeros((), device=device), torch.zeros(7, device=device), fresh(0), grad
-    loss, stats, logprobs = fresh(), fresh(7), fresh(tokens)
+    loss, stats, logprobs = fresh(()), fresh(7), fresh(tokens)
     entropies = fresh(tokens) if config.entropy_coef != 0.0 else None
     workspace = fresh(_size("lfm2_policy_workspace", tokens, sequences, int(cu_seqlens is not None)))
     _call_on(device, "lfm2_policy_gradient", loss, stats, logprobs, entropies, grad, _row_stride(grad), logits, _row_stride(logits),

@@ -466,3 +466,14 @@ def test_refusals_on_the_device(ops):
             bad()
     empty = ops.token_logprobs(logits[:0], targets[:0])
     assert empty.shape == (0,)
+
+
+def test_writing_the_gradient_over_logits_that_a_graph_saved_is_noticed(ops):
+    logits = torch.randn(3, 40, device=DEV, requires_grad=True)
+    targets = torch.tensor([1, 2, 3], device=DEV)
+    doubled = logits * 2
+    scores = ops.token_logprobs(doubled, targets)
+    _, _, stats = ops.token_logprobs_forward(doubled.detach(), targets)
+    ops.token_logprobs_backward(doubled.detach(), targets, stats, torch.ones(3, device=DEV), out=doubled.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        scores.sum().backward()
