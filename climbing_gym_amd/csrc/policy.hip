@@ -130,8 +130,8 @@ struct LogprobArgs {
 };
 
 // One workgroup per row; reads the row once.  stats[row] = (max, log s, entropy, 0) for the gradient.  Bound by reading:
-// 4096 rows of 65536 bf16 values (537 MB) take 77 us, 7.0 TB/s, as fast as this card reads anything; a call of a few rows is
-// the latency of one (6.5 us).
+// 4096 rows of 65536 bf16 values (537 MB) take 82 us, 6.6 TB/s (a loads-only kernel: 7.0); with entropies the vector unit is
+// about as busy as the memory (483 MB: 89 us, 5.4 TB/s).  A call of a few rows is the latency of one (6.5 us).
 template <typename T, int THREADS, bool ENTROPY, bool STREAM>
 __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(LogprobArgs a) {
   __shared__ float scratch[THREADS / 64];
@@ -214,7 +214,8 @@ struct BackwardArgs {
 constexpr int kBackwardVecs = 4;   // 16-byte pieces per thread
 
 // Elementwise given the row's statistics: workgroup (x, row) covers 256 * kBackwardVecs pieces of a row.  Bound by reading
-// and writing: 4096 rows of 65536 bf16 values (1.07 GB) take 188 us, 5.7 TB/s (a copy on this card: 4.7).
+// and writing: 4096 rows of 65536 bf16 values, a tenth of which does not count (1.02 GB), take 189 us, 5.4 TB/s (a copy on
+// this card: 4.7).
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(256) token_logprobs_backward_kernel(BackwardArgs a) {
   constexpr int VE = RowVec<T>::N;
@@ -598,7 +599,7 @@ template <typename V, int N> __device__ __forceinline__ void forget_unpacked(V (
 
 // One workgroup per row: statistics, the token's loss slope, and the row's gradient.  VECS > 0: the row is read once and
 // waits in registers (16 bytes each) while its statistics are joined; 0: a row too long for that is read twice.  Bound by
-// reading and writing: 8958 rows of 65536 bf16 values, of which a fifth does not count (2.1 GB), take 382 us, 5.5 TB/s.
+// reading and writing: 8958 rows of 65536 bf16 values, three tenths of which do not count (2.0 GB), take 381 us, 5.2 TB/s.
 // Whole calls (three to four launches), 4096 rows of 8192 / 32768 / 65536 values: 46 / 107 / 219 us, read twice 54 / 145 /
 // 270.  256 threads hold rows of up to 16 KiB: with 512, 4096 rows of 8192 values take 57.  1024 threads for the longest
 // rows that are held leave room for one row per CU at a time: 489 us for the 8958 rows, 406 with 512.
@@ -705,9 +706,11 @@ __global__ void __launch_bounds__(THREADS) policy_gradient_kernel(GradientArgs a
 }
 
 // ===================================================================================== host side
+constexpr int64_t kMostGroups = 1 << 22;   // workgroups of a launch: the threads of a grid are counted in 32 bits
 int check_logits(const char* name, int64_t N, int64_t V, int64_t stride) {
   LFM2_REQUIRE(N > 0 && V > 0, "%s: empty logits", name);
   LFM2_REQUIRE(N <= 0x7fffffff && V <= 0x7fffffff, "%s: at most 2^31 - 1 rows and columns", name);
+  LFM2_REQUIRE(N <= kMostGroups, "%s: more than 2^22 rows", name);
   LFM2_REQUIRE(stride >= V, "%s: rows overlap", name);
   return LFM2_OK;
 }
@@ -718,6 +721,7 @@ int fill_loss(const char* name, LossArgs* a, const float* logprobs, const float*
               float entropy_coef) {
   LFM2_REQUIRE(N > 0 && N <= 0x7fffffff, "%s: 1 to 2^31 - 1 tokens", name);
   LFM2_REQUIRE(!cu || (S > 0 && S <= 0x7fffffff), "%s: cu_seqlens needs at least one sequence", name);
+  LFM2_REQUIRE(!cu || S <= kMostGroups, "%s: more than 2^22 sequences", name);
   LFM2_REQUIRE(old && advantages, "%s: old log-probabilities and advantages are required", name);
   LFM2_REQUIRE(aggregate >= LFM2_MEAN_TOKENS && aggregate <= LFM2_MEAN_SUM, "%s: unknown aggregate %d", name, aggregate);
   LFM2_REQUIRE(kl >= LFM2_KL_K1 && kl <= LFM2_KL_K3, "%s: unknown KL estimator %d", name, kl);

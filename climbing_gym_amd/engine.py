@@ -588,6 +588,7 @@ class LFM25Engine:
         reject(share_prefix and self.dtype not in (torch.bfloat16, torch.float16), "shared prefixes need a bf16 or fp16 model")
         prompts = prefix.batch_size
         total = prompts * int(repeats)
+        reject(share_prefix and total > ops.MAX_SHARED_ROWS, f"more than {ops.MAX_SHARED_ROWS} rows share prefixes")
         cache_len = int(max_cache_len or prefix.cache.max_seq_len)
         reject(cache_len < prefix.cache.max_seq_len, "max_cache_len cannot be smaller than the prefix cache")
         cache = self._empty_cache(max_slots=total, max_seq_len=cache_len)

@@ -603,7 +603,8 @@ def attend_shared(q, k_cache, v_cache, k_scales, v_scales, positions, prefix: Sh
     in every row's slot, with one reading of the prefix per group and no copies (lfm25_engine.py:761 forks a prompt's cache
     once per completion).  Positions below `prefix.lengths[g]` are read from slot `prefix.slots[g]`, the others from the
     row's own slot, where the decode step appends them at their usual positions.  `schedule`: `shared_schedule` of the same
-    positions, prefix, mask and shapes (built here when None).  Slots or pages outside the cache give NaN rows."""
+    positions, prefix, mask and shapes (built here when None).  The scales of an e4m3 history are what `store_kv` writes: not
+    negative.  At most 4096 rows.  Slots or pages outside the cache give NaN rows."""
     reject(q.ndim != 4 or q.size(1) != 1 or q.dtype not in (torch.bfloat16, torch.float16), "queries must be bf16 or fp16 [rows, 1, heads, dim]")
     rows, _, query_heads, dim = q.shape
     reject(_check_batch_rows(positions, active, slot_ids) != rows, "positions must have one entry per row")
@@ -857,7 +858,7 @@ def token_logprobs_forward(logits: torch.Tensor, targets: torch.Tensor, *, tempe
     fp32 copy and runs logsumexp and gather: returns (log-probabilities fp32 [N], entropies fp32 [N] or None, row
     statistics fp32 [N, 4] for `token_logprobs_backward`).  `logits` [N, V] may be rows of a wider matrix; `targets` int64,
     a negative one takes its row out (zeros), one outside the vocabulary gives NaN; `temperature` a number or fp32 [N]
-    (rows with a temperature <= 0 are scored at 1).  Rows of -inf only give -inf and entropy 0."""
+    (rows with a temperature <= 0 are scored at 1).  Rows of -inf only give -inf and entropy 0.  At most 2^22 rows."""
     temperatures, value = _check_logits(logits, targets, temperature)
     device, rows = _one_device(logits, targets, temperatures), logits.size(0)
     logprobs = logits.new_empty(rows, dtype=torch.float32)

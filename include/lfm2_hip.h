@@ -274,7 +274,7 @@ int lfm2_shared_schedule(int32_t* schedule, const int32_t* positions, const uint
 int64_t lfm2_shared_schedule_size(int64_t B, int64_t capacity, int QH, int KH, int D);
 /* q, out [B,QH,D] bf16 or fp16; history in that type, or e4m3 with fp32 scales (kv_fp8; scales at the element's offset / D);
  * `pools` slots, or pages with block_table int32[B,max_blocks] (then c0 is the page stride); D in {32, 64, 128};
- * workspace: lfm2_shared_attention_workspace() floats. */
+ * workspace: lfm2_shared_attention_workspace() floats; scale > 0; a cache's tokens (c1) less than 2^23 elements apart. */
 int lfm2_shared_attention(void* out, const void* q, const void* k_cache, const void* v_cache, const float* k_scales, const float* v_scales,
                           const int32_t* schedule, const int32_t* block_table, int64_t max_blocks, int page, float* workspace,
                           int64_t B, int QH, int KH, int D, int64_t capacity, int64_t pools, int64_t c0, int64_t c1, int64_t c2,
@@ -387,7 +387,8 @@ int lfm2_record_head(const int64_t* ids, const float* probs, int32_t* out_ids, f
  *   stats float[N, 4] = (m, log s, entropy or NaN, 0): what the gradient needs.
  * Rows are V consecutive elements, row_stride elements apart, at any element alignment.  targets int64[N]: a negative
  * one takes its row out (zeros, the row is not read); one >= V gives NaN.  A row of -inf only has no distribution:
- * log-probability -inf, entropy 0.  NaN or +inf in a row makes its results NaN.  Sums in fp32. */
+ * log-probability -inf, entropy 0.  NaN or +inf in a row makes its results NaN.  Sums in fp32.  At most 2^22 rows here and
+ * in the other functions of this section that take logits, and 2^22 sequences. */
 int lfm2_token_logprobs(float* logprobs, float* entropy, float* stats, const void* logits, int64_t row_stride,
                         const int64_t* targets, const float* temperatures, float temperature, int64_t N, int64_t V, int dtype,
                         void* stream);

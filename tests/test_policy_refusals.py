@@ -104,3 +104,12 @@ def test_binding_signatures_match_the_header():
                 for name, args in re.findall(r"\b(?:int|int64_t)\s+(lfm2_\w+)\s*\(([^)]*)\)", text)}
     for name, signature in {**_lib._SIGNATURES, **_lib._INT64_RESULT}.items():
         assert declared[name] == signature, name
+
+
+def test_refuses_more_rows_or_sequences_than_a_launch_counts(library):
+    buffer = ctypes.create_string_buffer(4096)
+    p = ctypes.addressof(buffer)
+    many = (1 << 22) + 1
+    assert library.lfm2_token_logprobs(p, None, p, p, 8, p, None, 1.0, many, 8, 0, None) == -1 and b"2^22 rows" in library.lfm2_last_error()
+    assert library.lfm2_policy_loss(p, p, p, None, p, p, p, None, None, None, p, p, 4, many, 0, 0, 3, 0.2, 0.2, 0.0, 0.0, 0.0, None) == -1
+    assert b"2^22 sequences" in library.lfm2_last_error()

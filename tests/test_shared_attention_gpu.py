@@ -349,3 +349,10 @@ def test_refuses_tokens_too_far_apart(ops):
     ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
     with pytest.raises(ValueError, match="apart"):
         ops.attend_shared(torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device=DEV), cache, cache, None, None, ints(0), ops.SharedPrefix(ints(0, 1), ints(0), ints(1)))
+
+
+@pytest.mark.parametrize("scale", (0.0, -0.125, math.inf, math.nan))
+def test_refuses_scales_that_are_not_positive(ops, scale):
+    batch = Batch([(2, 10, 0)], (3,), seed=23)
+    with pytest.raises(ValueError, match="scale"):
+        batch.run(ops, scale=scale)
