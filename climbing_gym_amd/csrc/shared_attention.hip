@@ -561,13 +561,17 @@ template <bool PAGED> struct History {
   __device__ __forceinline__ History(const SharedArgs& args, int source, int h) : a(args), table_row(source) {
     bad = source < 0 || source >= a.sources;
     base = (PAGED || bad ? 0 : (int64_t)source * a.c0) + (int64_t)h * a.c2;
+    if (bad) table_row = -1;
   }
-  __device__ __forceinline__ int64_t offset(int t) {   // in elements
+  __device__ __forceinline__ int block_of(int t) const { return a.page_shift >= 0 ? t >> a.page_shift : t / a.page; }
+  __device__ __forceinline__ int page_of(int t) const {   // what the table says, checked when it is used
+    return table_row < 0 ? 0 : a.table[(int64_t)table_row * a.max_blocks + block_of(t)];
+  }
+  // in elements; `page` (paged only): page_of(t)
+  __device__ __forceinline__ int64_t offset(int t, int page = 0) {
     if constexpr (PAGED) {
-      const int block = a.page_shift >= 0 ? t >> a.page_shift : t / a.page;
-      int pool = bad ? 0 : a.table[(int64_t)table_row * a.max_blocks + block];
-      if (pool < 0 || pool >= a.pools) { bad = true; pool = 0; }
-      return base + (int64_t)pool * a.c0 + (int64_t)(t - block * a.page) * a.c1;
+      if (page < 0 || page >= a.pools) { bad = true; page = 0; }
+      return base + (int64_t)page * a.c0 + (int64_t)(t - block_of(t) * a.page) * a.c1;
     }
     return base + (int64_t)t * a.c1;
   }
@@ -586,7 +590,9 @@ template <typename T, bool FP8, int D> __device__ __forceinline__ void stage(bf1
 }
 
 // The way of K and V rows from memory to LDS: THREADS threads bring TOKENS tokens, consecutive threads consecutive 16-byte
-// pieces, so that every load instruction asks for whole cache lines.
+// pieces, so that every load instruction asks for whole cache lines.  Of a paged history, each lane looks one row of its
+// wave's up in the table, a tile ahead, and hands its place to the lanes that bring it: the table's latency in front of every
+// tile's own cost 55 rows of 128 dims and pages of 16 38 us of attention and join instead of 23.
 template <typename T, bool FP8, bool PAGED, int D, int THREADS, int TOKENS, bool STREAM> struct Rows {
   typedef Shape<T, FP8, D> S;
   static constexpr int N = TOKENS * S::ROW16 / THREADS;          // pieces per thread, of K and of V
@@ -597,10 +603,28 @@ template <typename T, bool FP8, bool PAGED, int D, int THREADS, int TOKENS, bool
   History<PAGED>& history;
   const int t1, thread, row_bytes;
   uint32_t whole[N];
-  __device__ __forceinline__ Rows(const SharedArgs& args, History<PAGED>& h, int end, int id)
-      : a(args), history(h), t1(end), thread(id), row_bytes((int)args.c1 * S::ES) {
+  // paged: rows of a wave per load instruction; the row this lane looks up; what it found for the next tile
+  static constexpr int PER = 64 / S::ROW16;
+  static_assert(PER * N <= 64 && THREADS % S::ROW16 == 0, "a wave has a lane for each of its rows");
+  const int own_row;
+  int page = 0, scale_page = 0;
+  // `first`: where the first fetch will be
+  __device__ __forceinline__ Rows(const SharedArgs& args, History<PAGED>& h, int first, int end, int id)
+      : a(args), history(h), t1(end), thread(id), row_bytes((int)args.c1 * S::ES),
+        own_row((id >> 6) * PER + (id & 63) % PER + THREADS / S::ROW16 * ((id & 63) / PER % N)) {
+    if constexpr (PAGED) {
+      look_up(first);
+    } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) whole[i] = row_of(i) * row_bytes + 16 * piece_of(i);
+      for (int i = 0; i < N; ++i) whole[i] = row_of(i) * row_bytes + 16 * piece_of(i);
+    }
+  }
+  // (a wave by itself looks up consecutive rows, so its lanes have the tokens of their scales already)
+  static constexpr bool SCALE_IS_OWN = THREADS == 64;
+  __device__ __forceinline__ void look_up(int T0) {
+    T0 = T0 < t1 ? T0 : t1 - 1;
+    page = history.page_of(T0 + min(own_row, t1 - 1 - T0));
+    if constexpr (FP8 && !SCALE_IS_OWN) scale_page = history.page_of(T0 + min(thread % TOKENS, t1 - 1 - T0));
   }
   __device__ __forceinline__ int row_of(int i) const { return (thread + THREADS * i) / S::ROW16; }
   __device__ __forceinline__ int piece_of(int i) const { return (thread + THREADS * i) % S::ROW16; }
@@ -610,18 +634,23 @@ template <typename T, bool FP8, bool PAGED, int D, int THREADS, int TOKENS, bool
     if constexpr (STREAM) return __builtin_nontemporal_load(p);
     else return *p;
   }
-  // tokens from T0 on, cut to the item's; past its end, its last token for every thread
-  __device__ __forceinline__ void fetch(int T0, Raw& x) {
+  // tokens from T0 on, cut to the item's; past its end, its last token for every thread.  The next fetch is of `next`.
+  __device__ __forceinline__ void fetch(int T0, int next, Raw& x) {
     T0 = T0 < t1 ? T0 : t1 - 1;
     const int last = t1 - 1 - T0;
     if constexpr (PAGED) {
+      const int64_t own = history.offset(T0 + min(own_row, last), page);
+      const int64_t bytes = own * S::ES;
+      const int low = (int)(uint32_t)bytes, high = (int)(bytes >> 32);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int64_t at = history.offset(T0 + min(row_of(i), last)) * S::ES + 16 * piece_of(i);
+        const int from = (thread & 63) / S::ROW16 + PER * i;
+        const int64_t at = (((int64_t)__shfl(high, from, 64) << 32) | (uint32_t)__shfl(low, from, 64)) + 16 * piece_of(i);
         x.k[i] = load(reinterpret_cast<const i32x4*>((const uint8_t*)a.kc + at));
         x.v[i] = load(reinterpret_cast<const i32x4*>((const uint8_t*)a.vc + at));
       }
-      if constexpr (FP8) load_scales(history.offset(T0 + min(thread % TOKENS, last)) / D, x);
+      if constexpr (FP8) load_scales((SCALE_IS_OWN ? own : history.offset(T0 + min(thread % TOKENS, last), scale_page)) / D, x);
+      look_up(next);
     } else {
       const int64_t start = history.offset(T0);
       const uint8_t* krows = (const uint8_t*)a.kc + start * S::ES;
@@ -680,10 +709,10 @@ __device__ __forceinline__ void block_item(const SharedArgs& a, const i32x4 r0, 
   const int t0 = r1[0] + (LONG ? wave * TOKENS : 0), t1 = r1[1];
   History<PAGED> history(a, PAGED && r1[3] == kOwn ? r0[0] : r1[2], h);
   typedef Rows<T, FP8, PAGED, D, 64, TOKENS, true> Tile;
-  Tile tile(a, history, t1, lane);
+  Tile tile(a, history, t0, t1, lane);
   typename Tile::Raw raw;
   const bool work = t0 < t1 && (PAGED || !history.bad);   // the same for the whole wave
-  if (work) tile.fetch(t0, raw);
+  if (work) tile.fetch(t0, t0 + STRIDE, raw);
   QueryBlock<T, FP8, D> block;
   block.start(a, r0, r1[3], h, r0[2] * kQueryBlock);
   if (work) {
@@ -697,7 +726,7 @@ __device__ __forceinline__ void block_item(const SharedArgs& a, const i32x4 r0, 
         tile.template stage_v<PART * COUNT, COUNT>(now, T0, lds_v);
         if constexpr (FP8 && PART == 0) tile.stage_scales(now, scales);
         wave_sync();
-        if constexpr (PART == PARTS - 1) tile.fetch(T0 + STRIDE, raw);
+        if constexpr (PART == PARTS - 1) tile.fetch(T0 + STRIDE, T0 + 2 * STRIDE, raw);
         if (PART == 0 || from < t1) attend_step<T, FP8, D, 2, 1>(a, &block, t1 - from, lds_k, lds_v, scales + kStep * PART);
       };
       part(std::integral_constant<int, 0>{});
@@ -742,10 +771,10 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const i32x4 r0,
   const int tokens = kShareTile / 4 * sets, first = wave / sets * tokens;   // the wave's share of a tile
   History<PAGED> history(a, r1[2], h);
   typedef Rows<T, FP8, PAGED, D, 256, kShareTile, false> Tile;
-  Tile tile(a, history, t1, threadIdx.x);
+  Tile tile(a, history, t0, t1, threadIdx.x);
   typename Tile::Raw raw;
   const bool readable = PAGED || !history.bad;
-  if (readable) tile.fetch(t0, raw);
+  if (readable) tile.fetch(t0, t0 + kShareTile, raw);
   Block blocks[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) blocks[n].start(a, r0, kShared, h, q0 + 16 * (NB * set + n));
@@ -756,7 +785,7 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const i32x4 r0,
       tile.template stage_v<0, Tile::N>(raw, T0, lds_v);
       if constexpr (FP8) tile.stage_scales(raw, scales);
       __syncthreads();
-      tile.fetch(T0 + kShareTile, raw);
+      tile.fetch(T0 + kShareTile, T0 + 2 * kShareTile, raw);
       for (int row = first; row < first + tokens; row += STEP) {
         const int from = T0 + row;
         if (from >= t1) break;
