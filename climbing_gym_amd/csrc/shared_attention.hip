@@ -11,7 +11,9 @@ namespace {
 constexpr float kInf = __builtin_huge_valf();
 constexpr int kStep = 32;                 // history tokens that meet 16 queries at a time
 constexpr int kShareTile = 4 * kStep;     // tokens a workgroup stages at a time of a part that a group shares
-constexpr int kGrain = 128;               // chunks are multiples of this
+// Chunks are multiples of this: those of a workgroup, those of a wave (128 for both: 16 rows of 900 tokens 12.4 us instead of
+// 11.2, six layers of 16 x 16 rows 318 instead of 308; 55 paged rows of 128 dims 36.7 instead of 38.4).
+constexpr int kGrain = 128, kWaveGrain = 64;
 constexpr int kMaxRows = 4096;            // rows and groups the work list holds
 constexpr int kSplitSlots = 2048;         // partial results beyond one per row and part, for each of the two chunk sizes
 constexpr int kQueryTile = 64;            // queries of an item that a group shares: its (row, head) pairs of one KV head
@@ -41,11 +43,11 @@ enum { kOwn, kShared, kCut };
 
 struct SlotBounds { int64_t slots, records; };
 // Upper bounds of the partial results and of the items of a batch, from what the host knows.  A row has at most
-// ceil(capacity / kGrain) shared and as many own chunks; a chunk size is at least 1 / kSplitSlots of the tokens it cuts (with
+// ceil(capacity / kWaveGrain) shared and as many own chunks; a chunk size is at least 1 / kSplitSlots of the tokens it cuts (with
 // multiplicity, the shared ones counted once per row), so each of the two sizes makes at most kSplitSlots chunks plus one
 // per part, and a row has two parts.  An item covers at least one row's queries, or a tile of them.
 SlotBounds slot_bounds(int64_t B, int64_t capacity, int G) {
-  const int64_t per_row = (capacity + kGrain - 1) / kGrain;
+  const int64_t per_row = (capacity + kWaveGrain - 1) / kWaveGrain;
   const int64_t half = B * per_row < B + kSplitSlots ? B * per_row : B + kSplitSlots;
   return SlotBounds{2 * half, 2 * half * ((G + kQueryBlock - 1) / kQueryBlock)};
 }
@@ -58,10 +60,31 @@ struct ScheduleArgs {
   const int32_t *positions, *slot_ids, *starts, *prefix_slots, *prefix_lengths;
   const uint8_t* active;
   int64_t capacity;
-  int B, groups, QH, KH, D;
+  int B, groups, QH, KH, G, D;
 };
 
 __device__ __forceinline__ int round_up(int v, int step) { return (v + step - 1) / step * step; }
+
+// How a part is cut: pieces of `tokens` tokens, a multiple of kWaveGrain.  The number of pieces goes through a float
+// reciprocal and an exact correction by one (an integer division is forty instructions, and this kernel has many).
+struct Cut {
+  int tokens, units;
+  float inverse;
+  static __device__ __forceinline__ Cut of(int size) {
+    return Cut{size, size / kWaveGrain, __builtin_amdgcn_rcpf((float)(size / kWaveGrain))};
+  }
+  // field by field: a choice between objects would put them into memory
+  static __device__ __forceinline__ Cut choose(bool first, const Cut a, const Cut b) {
+    return Cut{first ? a.tokens : b.tokens, first ? a.units : b.units, first ? a.inverse : b.inverse};
+  }
+  __device__ __forceinline__ int pieces(int n) const {   // ceil(n / tokens), n <= 2^28
+    const int x = (n + kWaveGrain - 1) / kWaveGrain + units - 1;
+    int q = (int)((float)x * inverse);
+    const int rest = x - q * units;
+    q += rest >= units ? 1 : rest < 0 ? -1 : 0;
+    return q;
+  }
+};
 
 // Four sums, and four exclusive prefix sums with their totals, over 1024 threads.
 __device__ __forceinline__ f32x4 sum4_1024(f32x4 v, f32x4* scratch) {
@@ -106,7 +129,7 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
   __shared__ int starts[MOST + 1], extent[MOST], source[MOST], prefix[MOST];
   __shared__ f32x4 fscratch[16];
   __shared__ i32x4 scratch[16];
-  const int tid = threadIdx.x, G = a.QH / a.KH, capacity = (int)a.capacity;
+  const int tid = threadIdx.x, G = a.G, capacity = (int)a.capacity;
   int length[PER], slot_of[PER], group[PER], shared[PER];   // shared: positions a row has in common with its group, 0: none
   bool cut[PER];
 #pragma unroll
@@ -188,23 +211,26 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
     else other_work += (float)extent[g];
   }
   const f32x4 sums = sum4_1024(f32x4{wide_tokens, other_tokens, wide_work, other_work}, fscratch);
-  auto chunk_of = [&](float tokens, float work, int items) {
+  auto chunk_of = [&](float tokens, float work, int items, int grain) {
     // a little more than the quotient: the sums are rounded.  (6e8 is above 2^40 tokens over kSplitSlots, and twice it an int.)
     const float need = fmaxf(tokens / (float)kSplitSlots, work * (float)a.KH / (float)items);
-    return round_up((int)fminf(need * 1.0001f, 6.0e8f) + 1, kGrain);
+    return round_up((int)fminf(need * 1.0001f, 6.0e8f) + 1, grain);
   };
-  // The shared parts' chunk: of sixteen sizes up to about twice the smallest that will do, the one whose longest workgroup is
-  // shortest (rounds of the workgroups times tokens, and what an item costs besides).  One wave tries one size.  (32 groups of
-  // 4 to 7 k tokens: 512 items of up to 3500 tokens instead of 640 of 2816, two rounds for a quarter of the workgroups.)
-  const int smallest = chunk_of(sums[0], sums[2], kSharedItems), step = round_up(smallest / 16 + 1, kGrain);
+  // The shared parts' chunk: of sixteen sizes up to about twice the smallest that will do, the one that is done first.  One
+  // wave tries one size.  Two workgroups on a CU do twice as many tokens in 1.4 of the time, and cost 256 tokens' time more
+  // than one (they start one after the other, and their partial results are written and joined): 16 x 16 rows, e4m3, 4000
+  // shared tokens as 512 items of 1024 take 35 us, as 256 of 2048 43; 4 x 16 rows, 2000 tokens, 512 of 128 19, 256 of 256 15;
+  // about 1000 tokens for each CU are done in the same time either way.
+  const int smallest = chunk_of(sums[0], sums[2], kSharedItems, kGrain), step = round_up(smallest / 16 + 1, kGrain);
   {
     const int wave = tid >> 6, chunk = smallest + wave * step;
+    const Cut cut = Cut::of(chunk);
     int items = 0;
     for (int g = tid & 63; g < a.groups; g += 64)
-      if (wide(g)) items += (extent[g] + chunk - 1) / chunk * ((queries(g) + kQueryTile - 1) / kQueryTile);
+      if (wide(g)) items += cut.pieces(extent[g]) * ((queries(g) + kQueryTile - 1) / kQueryTile);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) items += __shfl_xor(items, o, 64);
-    if ((tid & 63) == 0) scratch[wave][0] = __builtin_bit_cast(int, (float)((items * a.KH + kSharedBlocks - 1) / kSharedBlocks) * (float)(chunk + kGrain));
+    if ((tid & 63) == 0) scratch[wave][0] = __builtin_bit_cast(int, items * a.KH <= kTurn ? (float)chunk : (float)((items * a.KH + kSharedBlocks - 1) / kSharedBlocks) * (1.4f * (float)chunk + 256.f));
     __syncthreads();
   }
   int wide_chunk = smallest, least = scratch[0][0];   // positive floats are in order as integers too
@@ -214,27 +240,32 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
     if (cost < least) { least = cost; wide_chunk = smallest + c * step; }
   }
   __syncthreads();
-  const int other_chunk = chunk_of(sums[1], sums[3], kOwnItems);
+  const int short_chunk = chunk_of(sums[1], sums[3], kOwnItems, kWaveGrain);
+  const Cut wide_cut = Cut::of(wide_chunk), long_cut = Cut::of(round_up(short_chunk, kGrain)), short_cut = Cut::of(short_chunk);
   // a part's chunks, and its records by kind (0 shared, 1 long, 2 short)
-  struct Part { int chunk, chunks, records, kind; };
+  struct Part { int chunk, chunks, tiles, records, kind; };
   auto shared_part = [&](int g) {
     Part p;
-    p.chunk = wide(g) ? wide_chunk : other_chunk;
-    p.chunks = (extent[g] + p.chunk - 1) / p.chunk;
-    p.records = p.chunks * (wide(g) ? (queries(g) + kQueryTile - 1) / kQueryTile : 1);
     p.kind = wide(g) ? 0 : extent[g] > kWaveTokens ? 1 : 2;
+    const Cut cut = Cut::choose(p.kind == 0, wide_cut, Cut::choose(p.kind == 1, long_cut, short_cut));
+    p.chunk = cut.tokens;
+    p.chunks = cut.pieces(extent[g]);
+    p.tiles = wide(g) ? (queries(g) + kQueryTile - 1) / kQueryTile : 1;
+    p.records = p.chunks * p.tiles;
     return p;
   };
   auto own_part = [&](int tokens) {
     Part p;
-    p.chunk = other_chunk;
-    p.chunks = tokens > 0 ? (tokens + p.chunk - 1) / p.chunk : 0;
-    p.records = p.chunks * own_tiles;
     p.kind = tokens > kWaveTokens ? 1 : 2;
+    const Cut cut = Cut::choose(p.kind == 1, long_cut, short_cut);
+    p.chunk = cut.tokens;
+    p.chunks = tokens > 0 ? cut.pieces(tokens) : 0;
+    p.tiles = own_tiles;
+    p.records = p.chunks * own_tiles;
     return p;
   };
   // places: partial results of every row, then the records, kind after kind
-  int slots = 0, mine[3] = {0, 0, 0};
+  int slots = 0, shared_records = 0, long_records = 0, short_records = 0;
   int np[PER], ns[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -245,26 +276,27 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
       const Part own = own_part(length[i] - shared[i]);
       ns[i] = own.chunks;
       slots += np[i] + ns[i];
-      mine[1] += own.kind == 1 ? own.records : 0;
-      mine[2] += own.kind == 2 ? own.records : 0;
+      long_records += own.kind == 1 ? own.records : 0;
+      short_records += own.kind == 2 ? own.records : 0;
     }
     if (b < a.groups) {   // the same numbers once more, for groups
       const Part part = shared_part(b);
-#pragma unroll
-      for (int k = 0; k < 3; ++k) mine[k] += part.kind == k ? part.records : 0;
+      shared_records += part.kind == 0 ? part.records : 0;
+      long_records += part.kind == 1 ? part.records : 0;
+      short_records += part.kind == 2 ? part.records : 0;
     }
   }
   i32x4 totals;
-  const i32x4 first = scan4_1024(i32x4{mine[0], mine[1], mine[2], slots}, scratch, &totals);
-  int at[3] = {first[0], totals[0] + first[1], totals[0] + totals[1] + first[2]}, slot = first[3];
+  const i32x4 first = scan4_1024(i32x4{shared_records, long_records, short_records, slots}, scratch, &totals);
+  int shared_at = first[0], long_at = totals[0] + first[1], short_at = totals[0] + totals[1] + first[2], slot = first[3];
   int32_t* const records = a.schedule + kHeader + kRowInts * a.B;
-  auto put = [&](const Part& part, int row, int rows, int tiles, int offset, int t0, int end, int source, int whose) {
-    int& place = part.kind == 0 ? at[0] : part.kind == 1 ? at[1] : at[2];
-    for (int c = 0; c < part.chunks; ++c)
-      for (int qt = 0; qt < tiles; ++qt) {
-        i32x4* r = reinterpret_cast<i32x4*>(records + (int64_t)kRecordInts * place++);
+  // writes a part's records from `place` on
+  auto put = [&](const Part part, int place, int row, int rows, int offset, int t0, int end, int source, int whose) {
+    i32x4* r = reinterpret_cast<i32x4*>(records) + 2 * (int64_t)place;
+    for (int c = 0; c < part.chunks; ++c, t0 += part.chunk)
+      for (int qt = 0; qt < part.tiles; ++qt, r += 2) {
         r[0] = i32x4{row, rows, qt, offset + c};
-        r[1] = i32x4{t0 + c * part.chunk, min(t0 + (c + 1) * part.chunk, end), source, whose};
+        r[1] = i32x4{t0, min(t0 + part.chunk, end), source, whose};
       }
   };
 #pragma unroll
@@ -273,11 +305,18 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
     if (b < a.B) {
       *reinterpret_cast<i32x4*>(a.schedule + kHeader + kRowInts * b) = i32x4{slot, np[i], ns[i], length[i]};
       slot += np[i] + ns[i];
-      put(own_part(length[i] - shared[i]), b, 1, own_tiles, np[i], shared[i], length[i], slot_of[i], cut[i] ? kCut : kOwn);
+      const Part part = own_part(length[i] - shared[i]);
+      put(part, part.kind == 1 ? long_at : short_at, b, 1, np[i], shared[i], length[i], slot_of[i], cut[i] ? kCut : kOwn);
+      long_at += part.kind == 1 ? part.records : 0;
+      short_at += part.kind == 2 ? part.records : 0;
     }
     if (b < a.groups) {
       const Part part = shared_part(b);
-      if (part.chunks) put(part, starts[b], starts[b + 1] - starts[b], part.records / part.chunks, 0, 0, extent[b], source[b], kShared);
+      put(part, part.kind == 0 ? shared_at : part.kind == 1 ? long_at : short_at, starts[b], starts[b + 1] - starts[b], 0, 0, extent[b],
+          source[b], kShared);
+      shared_at += part.kind == 0 ? part.records : 0;
+      long_at += part.kind == 1 ? part.records : 0;
+      short_at += part.kind == 2 ? part.records : 0;
     }
   }
   if (tid == 0) {
@@ -945,7 +984,7 @@ int lfm2_shared_schedule(int32_t* schedule, const int32_t* positions, const uint
   LFM2_REQUIRE(schedule && positions && ((uintptr_t)schedule & 15) == 0, "shared_schedule: null or unaligned argument");
   LFM2_REQUIRE(groups > 0 && groups <= kMaxRows, "shared_schedule: 1 to %d groups", kMaxRows);
   LFM2_REQUIRE(starts && prefix_slots && prefix_lengths, "shared_schedule: the groups need bounds, slots and lengths");
-  const ScheduleArgs a{schedule, positions, slot_ids, starts, prefix_slots, prefix_lengths, active, capacity, (int)B, (int)groups, QH, KH, D};
+  const ScheduleArgs a{schedule, positions, slot_ids, starts, prefix_slots, prefix_lengths, active, capacity, (int)B, (int)groups, QH, KH, QH / KH, D};
   if (B <= 1024 && groups <= 1024) hipLaunchKernelGGL(shared_schedule_kernel<1>, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
   else hipLaunchKernelGGL(shared_schedule_kernel<kMaxRows / 1024>, dim3(1), dim3(1024), 0, (hipStream_t)stream, a);
   LFM2_LAUNCH_CHECK();
