@@ -15,17 +15,20 @@ constexpr int kShareTile = 4 * kStep;     // tokens a workgroup stages at a time
 // 11.2, six layers of 16 x 16 rows 318 instead of 308; 55 paged rows of 128 dims 36.7 instead of 38.4).
 constexpr int kGrain = 128, kWaveGrain = 64;
 constexpr int kMaxRows = 4096;            // rows and groups the work list holds
-constexpr int kSplitSlots = 2048;         // partial results beyond one per row and part, for each of the two chunk sizes
+constexpr int kSplitSlots = 2048;         // partial results beyond one per row and part, for the shared parts and for the others
 constexpr int kQueryTile = 64;            // queries of an item that a group shares: its (row, head) pairs of one KV head
 constexpr int kQueryBlock = 16;           // queries of the other items
 constexpr int kTurn = 256;                // workgroups, one per CU
 constexpr int kSharedBlocks = 2 * kTurn, kOtherBlocks = 3 * kTurn;
 constexpr int kSharedItems = 512;      // items the shared parts are cut into, if their length allows ...
-constexpr int kOwnItems = 2048;         // ... and the others
-// Up to this many tokens an item is one wave's, beyond it a workgroup's.  A workgroup's waves read four tiles in a row, which
-// the memory likes, and pay for their join.  512 rows with own parts of 256 / 500 / 1000 tokens: e4m3 46 / 70 / 125 us as
-// wave items, 55 / 79 / 127 as workgroup items; bf16 58 / 100 / 191 against 62 / 100 / 185; 256 rows of 2000: 176 against 169.
-constexpr int kWaveTokens = 1024;
+// ... and the others, as items of a wave and of a workgroup (256 rows with own parts of 2000 tokens, e4m3: 112 us with 2048
+// long items, 122 with 4096; six layers of 16 x 16 rows with up to 900: 282 us with 4096 short ones, 300 with 2048).
+constexpr int kShortItems = 4096, kLongItems = 2048;
+// Parts of up to this many tokens are waves' items, longer ones workgroups'.  A workgroup's waves read four tiles in a row, which
+// the memory likes, and pay for their join; waves' items fill the chip more evenly.  With 2048 instead of 1024: 4 x 16 rows with
+// own parts of 1 to 4000 tokens 57 us instead of 62 (e4m3: 47 instead of 53), 256 rows of 2000 181 instead of 177 (117, 113).
+// Waves' items alone: one row of 60000 54 us instead of 35, 64 rows of 6000 135 instead of 122.
+constexpr int kWaveTokens = 2048;
 
 // ---- the work list (int32), built once per decode step and used by every attention layer
 //   header: what the list was built for, number of records of each of the three kinds of item
@@ -44,8 +47,8 @@ enum { kOwn, kShared, kCut };
 struct SlotBounds { int64_t slots, records; };
 // Upper bounds of the partial results and of the items of a batch, from what the host knows.  A row has at most
 // ceil(capacity / kWaveGrain) shared and as many own chunks; a chunk size is at least 1 / kSplitSlots of the tokens it cuts (with
-// multiplicity, the shared ones counted once per row), so each of the two sizes makes at most kSplitSlots chunks plus one
-// per part, and a row has two parts.  An item covers at least one row's queries, or a tile of them.
+// multiplicity, the shared ones counted once per row), so the shared parts and the others make at most kSplitSlots chunks each
+// plus one per part, and a row has two parts.  An item covers at least one row's queries, or a tile of them.
 SlotBounds slot_bounds(int64_t B, int64_t capacity, int G) {
   const int64_t per_row = (capacity + kWaveGrain - 1) / kWaveGrain;
   const int64_t half = B * per_row < B + kSplitSlots ? B * per_row : B + kSplitSlots;
@@ -65,25 +68,26 @@ struct ScheduleArgs {
 
 __device__ __forceinline__ int round_up(int v, int step) { return (v + step - 1) / step * step; }
 
-// How a part is cut: pieces of `tokens` tokens, a multiple of kWaveGrain.  The number of pieces goes through a float
-// reciprocal and an exact correction by one (an integer division is forty instructions, and this kernel has many).
+// ceil(x / y) of positive numbers (x below 2^26) through a float reciprocal and an exact correction by one: an integer
+// division is forty instructions, and the work list's kernel has many.
+__device__ __forceinline__ int divide_up(int x, int y, float inverse) {
+  const int n = x + y - 1;
+  const int q = (int)((float)n * inverse), rest = n - q * y;
+  return q + (rest >= y ? 1 : rest < 0 ? -1 : 0);
+}
+__device__ __forceinline__ int divide_up(int x, int y) { return divide_up(x, y, __builtin_amdgcn_rcpf((float)y)); }
+// How parts are cut: into pieces of at most `units` times kWaveGrain tokens.
 struct Cut {
-  int tokens, units;
+  int units;
   float inverse;
   static __device__ __forceinline__ Cut of(int size) {
-    return Cut{size, size / kWaveGrain, __builtin_amdgcn_rcpf((float)(size / kWaveGrain))};
+    return Cut{size / kWaveGrain, __builtin_amdgcn_rcpf((float)(size / kWaveGrain))};
   }
   // field by field: a choice between objects would put them into memory
   static __device__ __forceinline__ Cut choose(bool first, const Cut a, const Cut b) {
-    return Cut{first ? a.tokens : b.tokens, first ? a.units : b.units, first ? a.inverse : b.inverse};
+    return Cut{first ? a.units : b.units, first ? a.inverse : b.inverse};
   }
-  __device__ __forceinline__ int pieces(int n) const {   // ceil(n / tokens), n <= 2^28
-    const int x = (n + kWaveGrain - 1) / kWaveGrain + units - 1;
-    int q = (int)((float)x * inverse);
-    const int rest = x - q * units;
-    q += rest >= units ? 1 : rest < 0 ? -1 : 0;
-    return q;
-  }
+  __device__ __forceinline__ int pieces(int tokens) const { return divide_up((tokens + kWaveGrain - 1) / kWaveGrain, units, inverse); }
 };
 
 // Four sums, and four exclusive prefix sums with their totals, over 1024 threads.
@@ -240,16 +244,23 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
     if (cost < least) { least = cost; wide_chunk = smallest + c * step; }
   }
   __syncthreads();
-  const int short_chunk = chunk_of(sums[1], sums[3], kOwnItems, kWaveGrain);
-  const Cut wide_cut = Cut::of(wide_chunk), long_cut = Cut::of(round_up(short_chunk, kGrain)), short_cut = Cut::of(short_chunk);
+  const Cut wide_cut = Cut::of(wide_chunk), long_cut = Cut::of(chunk_of(sums[1], sums[3], kLongItems, kGrain)),
+            short_cut = Cut::of(chunk_of(sums[1], sums[3], kShortItems, kWaveGrain));
   // a part's chunks, and its records by kind (0 shared, 1 long, 2 short)
-  struct Part { int chunk, chunks, tiles, records, kind; };
+  struct Part {
+    int chunk, chunks, tiles, records, kind;
+    // pieces of the same size: the longest decides when the launch is done
+    __device__ __forceinline__ void split(int tokens, const Cut cut, int grain) {
+      const int units = (tokens + kWaveGrain - 1) / kWaveGrain, most = max(cut.pieces(tokens), 1);
+      const int each = round_up(divide_up(units, most), grain / kWaveGrain);
+      chunk = each * kWaveGrain;
+      chunks = tokens > 0 ? divide_up(units, each) : 0;
+    }
+  };
   auto shared_part = [&](int g) {
     Part p;
     p.kind = wide(g) ? 0 : extent[g] > kWaveTokens ? 1 : 2;
-    const Cut cut = Cut::choose(p.kind == 0, wide_cut, Cut::choose(p.kind == 1, long_cut, short_cut));
-    p.chunk = cut.tokens;
-    p.chunks = cut.pieces(extent[g]);
+    p.split(extent[g], Cut::choose(p.kind == 0, wide_cut, Cut::choose(p.kind == 1, long_cut, short_cut)), p.kind == 2 ? kWaveGrain : kGrain);
     p.tiles = wide(g) ? (queries(g) + kQueryTile - 1) / kQueryTile : 1;
     p.records = p.chunks * p.tiles;
     return p;
@@ -257,9 +268,7 @@ __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
   auto own_part = [&](int tokens) {
     Part p;
     p.kind = tokens > kWaveTokens ? 1 : 2;
-    const Cut cut = Cut::choose(p.kind == 1, long_cut, short_cut);
-    p.chunk = cut.tokens;
-    p.chunks = tokens > 0 ? cut.pieces(tokens) : 0;
+    p.split(tokens, Cut::choose(p.kind == 1, long_cut, short_cut), p.kind == 2 ? kWaveGrain : kGrain);
     p.tiles = own_tiles;
     p.records = p.chunks * own_tiles;
     return p;
