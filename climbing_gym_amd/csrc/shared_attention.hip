@@ -910,7 +910,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 6
 
 // Joins the partial results of one (row, query head) per wave: weights 2^{m_c - max}, one chunk per lane, read back lane by
 // lane; lanes own dims.  The results were written by other XCDs and come from beyond the local L2: what counts is the
-// number of dependent loads, so a chunk's maximum and sum are read together, and the results of eight chunks at a time.
+// number of dependent loads, so a chunk's maximum and sum are read together with the first results, eight chunks at a time.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) shared_combine_kernel(SharedArgs a) {
   constexpr int PER = (D + 63) / 64, BATCH = 8;
@@ -929,6 +929,16 @@ __global__ void __launch_bounds__(256) shared_combine_kernel(SharedArgs a) {
   float top = -kInf, lt = 0.f, o[PER] = {};
   for (int c0 = 0; c0 < n; c0 += 64) {
     const int here = min(64, n - c0);
+    float v[BATCH][PER];
+    auto fetch = [&](int i0) {
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const float* from = a.acc + (first + (int64_t)(c0 + min(i0 + i, here - 1)) * a.QH) * D;
+#pragma unroll
+        for (int u = 0; u < PER; ++u) v[i][u] = from[min(lane + 64 * u, D - 1)];
+      }
+    };
+    fetch(0);
     const int64_t mine = first + (int64_t)(c0 + min(lane, here - 1)) * a.QH;
     const float mc = lane < here ? a.m[mine] : -kInf, lc = a.l[mine];
     const float now = fmaxf(top, wave_max(mc)), before = now == -kInf ? 1.f : __builtin_amdgcn_exp2f(top - now);
@@ -938,13 +948,7 @@ __global__ void __launch_bounds__(256) shared_combine_kernel(SharedArgs a) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) o[u] *= before;
     for (int i0 = 0; i0 < here; i0 += BATCH) {
-      float v[BATCH][PER];
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const float* from = a.acc + (first + (int64_t)(c0 + min(i0 + i, here - 1)) * a.QH) * D;
-#pragma unroll
-        for (int u = 0; u < PER; ++u) v[i][u] = from[min(lane + 64 * u, D - 1)];
-      }
+      if (i0) fetch(i0);
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
         // chunks past the last: weight 0, of a value that was read before and is not used
