@@ -477,3 +477,46 @@ def test_writing_the_gradient_over_logits_that_a_graph_saved_is_noticed(ops):
     ops.token_logprobs_backward(doubled.detach(), targets, stats, torch.ones(3, device=DEV), out=doubled.detach())
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         scores.sum().backward()
+
+
+@pytest.mark.parametrize("sequences", (2047, 2048, 2049, 4096))
+def test_many_sequences_over_few_tokens(ops, sequences):
+    n = 4096
+    lp, old, a, mask, _, _ = _tokens(n, sequences)
+    g = torch.Generator().manual_seed(sequences)
+    bounds = [0, *torch.randint(0, n + 1, (sequences - 1,), generator=g).sort().values.tolist(), n - 1]
+    bounds[-1] = max(bounds[-1], bounds[-2])
+    cfg = ops.PolicyLossConfig(aggregate="sequence")
+    x = lp.double().requires_grad_()
+    want, stats = _definition(x, old.double(), a.double(), mask, None, None, bounds, cfg)
+    want_g, = torch.autograd.grad(want, x)
+    got = ops.policy_loss_forward(lp.to(DEV), old.to(DEV), a.to(DEV), mask=mask.to(DEV), config=cfg,
+                                  cu_seqlens=torch.tensor(bounds, dtype=torch.int32).to(DEV))
+    _compare_loss(got[:3], want.detach(), stats, want_g, (want_g.abs().sum() + stats[:3].abs().sum() + 1).item())
+
+
+@pytest.mark.parametrize("rows", (65535, 65536, 131071))
+def test_more_rows_than_one_grid_dimension_holds(ops, rows):
+    logits, targets = _rows(rows, 3, torch.float32, rows)
+    targets[::7] = -1
+    lp, h, stats = ops.token_logprobs_forward(logits, targets, entropy=True)
+    _check_forward(lp, h, logits, targets, 1.0)
+    g = torch.randn(rows, generator=torch.Generator().manual_seed(1)).to(DEV)
+    _check_grad(ops.token_logprobs_backward(logits, targets, stats, g, g.flip(0)), logits, targets, g, g.flip(0), 1.0)
+
+
+def test_rows_further_apart_than_32_bits_count(ops):
+    """Rows 2^31 elements apart: the last one starts 8 GiB behind the first."""
+    stride, v = 1 << 31, 4097
+    storage = torch.empty(2 * stride + v, dtype=torch.bfloat16, device=DEV)
+    logits = storage.as_strided((3, v), (stride, 1))
+    near, targets = _rows(3, v, torch.bfloat16, 9)
+    logits.copy_(near)
+    ones = torch.ones(3, device=DEV)
+    got = ops.token_logprobs_forward(logits, targets)
+    want = ops.token_logprobs_forward(near, targets)
+    assert torch.equal(got[0], want[0])
+    grad = ops.token_logprobs_backward(near, targets, want[2], ones)
+    fused = ops.policy_gradient(near, targets, want[0] - 0.1, ones)
+    assert torch.equal(ops.policy_gradient(logits, targets, want[0] - 0.1, ones)[3], fused[3])
+    assert torch.equal(ops.token_logprobs_backward(logits, targets, got[2], ones, out=logits), grad)

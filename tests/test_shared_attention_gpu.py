@@ -356,3 +356,52 @@ def test_refuses_scales_that_are_not_positive(ops, scale):
     batch = Batch([(2, 10, 0)], (3,), seed=23)
     with pytest.raises(ValueError, match="scale"):
         batch.run(ops, scale=scale)
+
+
+def test_groups_may_share_one_slot(ops):
+    batch = Batch([(3, 100, 0), (4, 100, 0)], (5, 40), seed=24)
+    batch.prefix_args[1][1] = batch.prefix_args[1][0]
+    batch.leader[3:7] = [0] * 4
+    batch.check(ops)
+
+
+def test_slots_further_apart_than_32_bits_count(ops):
+    """Slots 2^31 elements apart: the third one starts 8 GiB behind the first."""
+    batch = Batch([(2, 200, 1), (1, 40, 0)], (9, 70), heads=(8, 2), seed=25)
+    slots, cap, heads, dim = batch.dk.shape
+    far = []
+    for t in (batch.dk, batch.dv):
+        storage = torch.empty((slots - 1) * (1 << 31) + heads * cap * dim, dtype=t.dtype, device=DEV)
+        view = storage.as_strided((slots, cap, heads, dim), (1 << 31, dim, cap * dim, 1))
+        view.copy_(t)
+        far.append(view)
+    near = batch.check(ops)
+    batch.dk, batch.dv = far
+    assert torch.equal(batch.run(ops), near)
+
+
+def test_two_graphs_of_one_pool_and_a_side_stream(ops):
+    first = Batch([(6, 200, 0), (4, 77, 0)], (150, 3), fp8=True, seed=26)
+    second = Batch([(20, 300, 0)], (1, 64), dim=128, seed=27)
+    want = [b.check(ops) for b in (first, second)]
+    graphs, held = [], []
+    for b in (first, second):
+        q = b.q.to(DEV)
+        call = lambda: ops.attend_shared(q, b.dk, b.dv, b.dks, b.dvs, b.positions, ops.SharedPrefix(*b.prefix_args))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0][0].pool() if graphs else None):
+            held.append(call())
+        graphs.append((graph, q))
+    for turn in (0, 1, 0, 0, 1, 1, 0):
+        graphs[turn][0].replay()
+        eager = (first, second)[1 - turn].run(ops)
+        torch.cuda.synchronize()
+        assert torch.equal(held[turn], want[turn]) and torch.equal(eager, want[1 - turn])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = first.run(ops)
+    other = second.run(ops)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want[0]) and torch.equal(other, want[1])
