@@ -603,19 +603,18 @@ def attend_shared(q, k_cache, v_cache, k_scales, v_scales, positions, prefix: Sh
     in every row's slot, with one reading of the prefix per group and no copies (lfm25_engine.py:761 forks a prompt's cache
     once per completion).  Positions below `prefix.lengths[g]` are read from slot `prefix.slots[g]`, the others from the
     row's own slot, where the decode step appends them at their usual positions.  `schedule`: `shared_schedule` of the same
-    positions, prefix, mask and shapes (built here when None).  The scales of an e4m3 history are what `store_kv` writes: not
-    negative.  At most 4096 rows.  Slots or pages outside the cache give NaN rows."""
+    positions, prefix, mask and shapes (built here when None; when given, it alone says what they say).  The scales of an
+    e4m3 history are what `store_kv` writes: not negative.  At most 4096 rows.  Slots or pages outside the cache give NaN
+    rows."""
     reject(q.ndim != 4 or q.size(1) != 1 or q.dtype not in (torch.bfloat16, torch.float16), "queries must be bf16 or fp16 [rows, 1, heads, dim]")
     rows, _, query_heads, dim = q.shape
     reject(_check_batch_rows(positions, active, slot_ids) != rows, "positions must have one entry per row")
-    prefix.check()
-    device = _one_device(q, k_cache, v_cache, k_scales, v_scales, positions, prefix.starts, prefix.slots, prefix.lengths, active,
-                         slot_ids, block_table, schedule)
+    device = _one_device(q, k_cache, v_cache, k_scales, v_scales, positions, active, slot_ids, block_table, schedule)
     reject(not q.is_contiguous(), "HIP kernels require contiguous tensors")
     strides = _cache_strides(k_cache)
     pools, _, heads, width = k_cache.shape
     fp8 = k_scales is not None
-    reject(width != dim or v_cache.shape != k_cache.shape or _cache_strides(v_cache) != strides, "key and value caches must match each other and the head dim")
+    reject(width != dim or v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride(), "key and value caches must match each other and the head dim")
     reject(k_cache.dtype != (FP8 if fp8 else q.dtype) or v_cache.dtype != k_cache.dtype, "the history is e4m3 with scales, or of the queries' type without")
     reject(heads == 0 or query_heads % heads, "query heads must be a multiple of the KV heads")
     reject(fp8 != (v_scales is not None), "an e4m3 history needs both scale tensors")
@@ -633,6 +632,7 @@ def attend_shared(q, k_cache, v_cache, k_scales, v_scales, positions, prefix: Sh
         capacity = block_table.size(1) * page
     if schedule is None:
         schedule = shared_schedule(positions, prefix, active, slot_ids, capacity=capacity, query_heads=query_heads, kv_heads=heads, head_dim=dim)
+        reject(schedule.device != device, "all tensors of a call live on one device")
     else:
         reject(schedule.dtype != torch.int32 or not schedule.is_contiguous()
                or schedule.numel() < _size("lfm2_shared_schedule_size", rows, capacity, query_heads, heads, dim),
