@@ -127,6 +127,7 @@ __device__ __forceinline__ i32x4 scan4_1024(const i32x4 v, i32x4* scratch, i32x4
 
 // One workgroup.  A thread has PER rows and PER groups (one each up to 1024 of them).  Its time is that of its dependent
 // rounds: everything is read from memory at the start, at once, and the sums and places of all kinds go through two joins.
+// 8 us up to 1024 rows, 16 to 22 for 2048 to 4096 (4096 groups of one row: 37).
 template <int PER>
 __global__ void __launch_bounds__(1024) shared_schedule_kernel(ScheduleArgs a) {
   constexpr int MOST = 1024 * PER;
@@ -864,6 +865,10 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const i32x4 r0,
   }
 }
 
+// Own parts alone (256 rows of 2000 tokens, 8 KV heads of 64 dims): 177 us in bf16, 6.1 TB/s; 113 in e4m3, 5.1 TB/s, where
+// the three waves a SIMD has registers for do not ask for enough bytes.  Shared parts alone (32 x 16 rows, 5500 tokens, 23
+// GFLOP, 90 M exponentials): 77 and 70 us with the join, bound by LDS reads and vector
+// instructions per score (e4m3: loads alone 45, arithmetic alone 56, with staging 65).
 template <typename T, bool FP8, bool PAGED, int D>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3 : 2))) shared_attention_kernel(SharedArgs a) {
   typedef Shape<T, FP8, D> S;
@@ -910,7 +915,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 6
 
 // Joins the partial results of one (row, query head) per wave: weights 2^{m_c - max}, one chunk per lane, read back lane by
 // lane; lanes own dims.  The results were written by other XCDs and come from beyond the local L2: what counts is the
-// number of dependent loads, so a chunk's maximum and sum are read together with the first results, eight chunks at a time.
+// number of dependent loads, so a chunk's maximum and sum are read together with the first results, eight chunks at a time
+// (512 rows of 32 heads: 7.5 us; 256 rows: 5.4).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) shared_combine_kernel(SharedArgs a) {
   constexpr int PER = (D + 63) / 64, BATCH = 8;
