@@ -64,6 +64,17 @@ def graph_capacity(cache_len: int, batch_size: int, max_model_len: int) -> int:
     return min(max_model_len, -(-cache_len // step) * step)
 
 
+def _hold_generator_state(device):
+    """An empty graph that has the device's generator registered, to be kept as long as captures may follow.  The seed and
+    offset that all live captures share are made for the first graph that registers and written at the beginning of every
+    capture.  Captures of this package run in inference mode; tensors made there may not be written outside of it, so the
+    next capture of the program around it would be refused.  Made here they are ordinary ones, which both may write."""
+    with torch.inference_mode(False), torch.cuda.device(device):
+        graph = torch.cuda.CUDAGraph()
+        graph.register_generator_state(torch.cuda.default_generators[torch.cuda.current_device()])
+    return graph
+
+
 class LFM25HIPDecoder:
     def __init__(self, engine, *, max_graphs: int = 2, max_prefill_tokens: int = 4096, finish_check_interval: int = 32,
                  skip_finished_attention: bool = True, fp8_mlp: bool = False, fp8_kv: bool = False,
@@ -90,6 +101,7 @@ class LFM25HIPDecoder:
         self._active_session = None
         # One stream for every capture of this decoder's lifetime (captures may come from different host threads).
         self._capture_stream = torch.cuda.Stream(device=engine.device)
+        self._generator_state = _hold_generator_state(engine.device) if self.capture else None
         self._prepare_fp8_weights()
 
     # ------------------------------------------------------------------ weights
