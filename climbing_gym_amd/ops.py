@@ -927,6 +927,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, temperature=1
     """`token_logprobs_forward` for autograd: log-probabilities, or (log-probabilities, entropies), differentiable in the
     logits (once; the temperature is a constant).  Inside a graph capture use the explicit pair."""
     _refuse_captured_graph(logits)
+    if torch.is_grad_enabled() and logits.requires_grad:   # a graph keeps no tensor of inference mode, as the engine's tokens are
+        targets, temperature = [t.clone() if isinstance(t, torch.Tensor) and t.is_inference() else t for t in (targets, temperature)]
     return _TokenLogprobs.apply(logits, targets, temperature, bool(entropy))
 
 
