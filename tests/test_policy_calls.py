@@ -24,6 +24,7 @@ def test_tokens_and_temperatures_that_inference_made_go_through_autograd():
     assert targets.is_inference() and temperature.is_inference()
     for a, b in zip(grads(targets, temperature), want):
         assert torch.equal(a, b)
+    with torch.inference_mode():
         scores = host.to(DEV)
     assert scores.is_inference() and torch.equal(ops.token_logprobs(scores, targets, temperature=temperature), want[0])   # no graph
     with torch.inference_mode():      # the losses' arguments from inference too
