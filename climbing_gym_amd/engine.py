@@ -160,6 +160,13 @@ def prefix_of_repeats(prompts: int, repeats: int, prompt_lengths: torch.Tensor) 
     return ops.SharedPrefix(bounds, bounds[:-1].clone(), prompt_lengths.to(torch.int32).clone())
 
 
+def _plain_rows(name: str, values) -> list:
+    """Sequences, arrays and tensors (of them) as a list of numbers and of lists of numbers."""
+    reject(values is None, f'{name} must match the completions')
+    plain = lambda v: v.tolist() if hasattr(v, 'tolist') else v
+    return [[float(plain(x)) for x in row] if hasattr(row, '__len__') else float(row) for row in map(plain, plain(values))]
+
+
 class LFM25Engine:
     def __init__(self, weights: LFM25PackedWeights, *, max_model_len: int | None = None) -> None:
         reject(weights.device.type != "cuda", "this engine runs on the GPU only; weights must live on a HIP device")
@@ -727,19 +734,24 @@ class LFM25Engine:
         """The clipped policy loss of sampled completions under the weights the engine holds now, for instance after
         `sync_from_model`: how far the policy has moved from the one that drew them.  `old_logprobs` (and `ref_logprobs`):
         per completion, one value per token, at the sampling temperature; `advantages`: one number per completion, or one
-        per token like these."""
+        per token like these.  Sequences, arrays and tensors, or sequences of them."""
         lengths = [len(c) for c in completions]
         reject(not lengths, 'an objective needs at least one completion')
-        per_sequence = len(advantages) > 0 and not hasattr(advantages[0], '__len__')
-        flat = {}
-        for name, values, wanted in (('old_logprobs', old_logprobs, lengths), ('ref_logprobs', ref_logprobs, lengths),
-                                     ('advantages', advantages, None if per_sequence else lengths)):
-            if values is None:
-                continue
-            reject(len(values) != len(lengths) or (wanted is not None and [len(v) for v in values] != wanted),
-                   f'{name} must match the completions')
-            numbers = [float(x) for x in values] if wanted is None else [float(x) for v in values for x in v]
-            flat[name] = torch.tensor(numbers, dtype=torch.float32).to(self.device)
+        reject(config.kl_coef != 0.0 and ref_logprobs is None, 'a KL term needs ref_logprobs')
+        temperature = ops._temperature_number(temperature)
+        advantages = _plain_rows('advantages', advantages)
+        per_sequence = not any(isinstance(row, list) for row in advantages)
+        per_token = [('old_logprobs', _plain_rows('old_logprobs', old_logprobs))]
+        if ref_logprobs is not None:
+            per_token.append(('ref_logprobs', _plain_rows('ref_logprobs', ref_logprobs)))
+        if not per_sequence:
+            per_token.append(('advantages', advantages))
+        reject(len(advantages) != len(lengths), 'advantages must match the completions')
+        flat = {'advantages': advantages}
+        for name, rows in per_token:
+            reject([len(row) if isinstance(row, list) else None for row in rows] != lengths, f'{name} must match the completions')
+            flat[name] = [number for row in rows for number in row]
+        flat = {name: torch.tensor(numbers, dtype=torch.float32).to(self.device) for name, numbers in flat.items()}
         bounds = [0, *itertools.accumulate(lengths)]
         logprobs = torch.empty(bounds[-1], device=self.device, dtype=torch.float32)
         entropy = torch.empty_like(logprobs) if config.entropy_coef != 0.0 else None

@@ -825,8 +825,12 @@ def _check_logits(logits, targets, temperature):
     if isinstance(temperature, torch.Tensor):
         _check_row_values(temperature, logits.size(0), torch.float32, "temperature")
         return temperature, 1.0
+    return None, _temperature_number(temperature)
+
+
+def _temperature_number(temperature) -> float:
     reject(not 0.0 < float(temperature) < float("inf"), "temperature must be positive and finite, or an fp32 tensor with one entry per row")
-    return None, float(temperature)
+    return float(temperature)
 
 
 def _check_row_values(tensor, rows: int, dtype, name: str) -> None:
