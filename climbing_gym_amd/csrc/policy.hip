@@ -8,12 +8,11 @@ namespace {
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_huge_valf();
 
-#define DISPATCH_LOGITS(dtype, name, ...)                                                  \
-  switch (dtype) {                                                                         \
+#define DISPATCH_LOGITS(dtype, ...)                                                        \
+  switch (dtype) {   /* check_scoring has seen it */                                       \
     case LFM2_DTYPE_BF16: { typedef __bf16 T; __VA_ARGS__; } break;                        \
     case LFM2_DTYPE_F16: { typedef _Float16 T; __VA_ARGS__; } break;                       \
     case LFM2_DTYPE_F32: { typedef float T; __VA_ARGS__; } break;                          \
-    default: LFM2_FAIL(LFM2_ERR_UNSUPPORTED, "%s: dtype %d is not bf16/f16/f32", name, dtype); \
   }
 
 // Sixteen bytes of a row.  A row of an odd vocabulary, or one inside a padded matrix, starts at any multiple of the
@@ -706,6 +705,14 @@ __global__ void __launch_bounds__(THREADS) policy_gradient_kernel(GradientArgs a
 }
 
 // ===================================================================================== host side
+// The type, and the number that divides the logits: log2(e) / temperature has to be a finite float.
+int check_scoring(const char* name, const float* temperatures, float temperature, int dtype) {
+  LFM2_REQUIRE(temperatures || (temperature >= __FLT_MIN__ && temperature <= __FLT_MAX__), "%s: temperature must be a positive normal number", name);
+  if (dtype != LFM2_DTYPE_BF16 && dtype != LFM2_DTYPE_F16 && dtype != LFM2_DTYPE_F32)
+    LFM2_FAIL(LFM2_ERR_UNSUPPORTED, "%s: dtype %d is not bf16/f16/f32", name, dtype);
+  return LFM2_OK;
+}
+bool finite(float v) { return v >= -__FLT_MAX__ && v <= __FLT_MAX__; }
 constexpr int64_t kMostGroups = 1 << 22;   // workgroups of a launch: the threads of a grid are counted in 32 bits
 int check_logits(const char* name, int64_t N, int64_t V, int64_t stride) {
   LFM2_REQUIRE(N > 0 && V > 0, "%s: empty logits", name);
@@ -726,7 +733,8 @@ int fill_loss(const char* name, LossArgs* a, const float* logprobs, const float*
   LFM2_REQUIRE(aggregate >= LFM2_MEAN_TOKENS && aggregate <= LFM2_MEAN_SUM, "%s: unknown aggregate %d", name, aggregate);
   LFM2_REQUIRE(kl >= LFM2_KL_K1 && kl <= LFM2_KL_K3, "%s: unknown KL estimator %d", name, kl);
   LFM2_REQUIRE(clip_low >= 0.f && clip_low < 1.f && clip_high >= 0.f && clip_high <= 3.0e38f, "%s: clip range outside [0, 1) x [0, inf)", name);
-  LFM2_REQUIRE(dual_clip == 0.f || dual_clip > 1.f, "%s: dual_clip is 0 (off) or above 1", name);
+  LFM2_REQUIRE(dual_clip == 0.f || (dual_clip > 1.f && finite(dual_clip)), "%s: dual_clip is 0 (off) or above 1", name);
+  LFM2_REQUIRE(finite(kl_coef) && finite(entropy_coef), "%s: coefficients must be finite", name);
   *a = LossArgs{logprobs, old, advantages, ref, entropy, mask, targets, cu, nullptr, N, cu ? S : 1, cu ? S : 1, per_sequence, aggregate, kl,
                 clip_low, clip_high, dual_clip, kl_coef, entropy_coef, __builtin_log1p(-(double)clip_low),
                 __builtin_log1p((double)clip_high), dual_clip > 0.f ? __builtin_log((double)dual_clip) : 0.0};
@@ -775,12 +783,12 @@ int lfm2_token_logprobs(float* logprobs, float* entropy, float* stats, const voi
   const int bad = check_logits("token_logprobs", N, V, row_stride);
   if (bad) return bad;
   LFM2_REQUIRE(logprobs && stats && logits && targets, "token_logprobs: null argument");
-  LFM2_REQUIRE(temperatures || temperature > 0.f, "token_logprobs: temperature must be positive");
+  if (int e = check_scoring("token_logprobs", temperatures, temperature, dtype)) return e;
   const LogprobArgs a{logprobs, entropy, stats, logits, targets, temperatures, row_stride, V, temperature};
   hipStream_t s = (hipStream_t)stream;
 #define LOGPROBS_(THREADS, ENTROPY, STREAM) \
   hipLaunchKernelGGL((token_logprobs_kernel<T, THREADS, ENTROPY, STREAM>), dim3((unsigned)N), dim3(THREADS), 0, s, a)
-  DISPATCH_LOGITS(dtype, "token_logprobs",
+  DISPATCH_LOGITS(dtype,
     // 4096 rows of 4096 / 8192 values: 7.7 / 14.5 us with 128 threads, 11.7 / 16.2 with 512; of 65536: 85 and 83; 64 rows of
     // 16384: 5.2 and 4.2
     const bool stream_once = N * row_stride * (int64_t)sizeof(T) >= kStreamBytes;
@@ -802,11 +810,11 @@ int lfm2_token_logprobs_backward(void* grad, int64_t grad_stride, const void* lo
   if (!bad) bad = check_logits("token_logprobs_backward", N, V, grad_stride);
   if (bad) return bad;
   LFM2_REQUIRE(grad && stats && logits && targets && grad_logprobs, "token_logprobs_backward: null argument");
-  LFM2_REQUIRE(temperatures || temperature > 0.f, "token_logprobs_backward: temperature must be positive");
+  if (int e = check_scoring("token_logprobs_backward", temperatures, temperature, dtype)) return e;
   const BackwardArgs a{grad, logits, targets, stats, grad_logprobs, grad_entropy, temperatures, grad_stride, row_stride, V, temperature};
   hipStream_t s = (hipStream_t)stream;
   // a grid's y holds 65535 rows
-  DISPATCH_LOGITS(dtype, "token_logprobs_backward",
+  DISPATCH_LOGITS(dtype,
     const int64_t pieces = V / RowVec<T>::N;
     const unsigned x = (unsigned)(pieces ? (pieces + 256 * kBackwardVecs - 1) / (256 * kBackwardVecs) : 1);
     for (int64_t row = 0; row < N; row += 65535) {
@@ -858,7 +866,8 @@ int lfm2_policy_gradient(float* loss, float* stats, float* logprobs, float* entr
   if (bad) return bad;
   LFM2_REQUIRE(loss && stats && logprobs && grad && logits && targets && workspace, "policy_gradient: null argument");
   LFM2_REQUIRE(entropy_coef == 0.f || entropy, "policy_gradient: an entropy term needs the entropy output");
-  LFM2_REQUIRE(temperatures || temperature > 0.f, "policy_gradient: temperature must be positive");
+  LFM2_REQUIRE(finite(grad_scale), "policy_gradient: grad_scale must be finite");
+  if (int e = check_scoring("policy_gradient", temperatures, temperature, dtype)) return e;
   g.logprobs = logprobs; g.entropy = entropy; g.grad = grad; g.logits = logits; g.temperatures = temperatures;
   g.grad_stride = grad_stride; g.stride = row_stride; g.V = V; g.temperature = temperature; g.grad_scale = grad_scale;
   hipStream_t s = (hipStream_t)stream;
@@ -869,7 +878,7 @@ int lfm2_policy_gradient(float* loss, float* stats, float* logprobs, float* entr
     if (entropy) hipLaunchKernelGGL((policy_gradient_kernel<T, THREADS, VECS, true>), dim3((unsigned)N), dim3(THREADS), 0, s, g);  \
     else hipLaunchKernelGGL((policy_gradient_kernel<T, THREADS, VECS, false>), dim3((unsigned)N), dim3(THREADS), 0, s, g);         \
   } while (0)
-  DISPATCH_LOGITS(dtype, "policy_gradient",
+  DISPATCH_LOGITS(dtype,
     const int64_t pieces = V / RowVec<T>::N;
     if (pieces <= 256 * 4) GRADIENT_(256, 4);
     else if (pieces <= 512 * 8) GRADIENT_(512, 8);

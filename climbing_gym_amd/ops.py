@@ -828,8 +828,13 @@ def _check_logits(logits, targets, temperature):
     return None, _temperature_number(temperature)
 
 
+_FP32 = torch.finfo(torch.float32)
+
+
 def _temperature_number(temperature) -> float:
-    reject(not 0.0 < float(temperature) < float("inf"), "temperature must be positive and finite, or an fp32 tensor with one entry per row")
+    # (logits are multiplied by log2(e) / temperature, which has to be finite too)
+    reject(not _FP32.tiny <= float(temperature) <= _FP32.max,
+           "temperature must be a positive normal number of fp32, or an fp32 tensor with one entry per row")
     return float(temperature)
 
 
@@ -861,8 +866,8 @@ def token_logprobs_forward(logits: torch.Tensor, targets: torch.Tensor, *, tempe
     """log softmax(logits / temperature) at `targets` in one pass over the logits, where lfm25_engine.py:1108-1163 makes an
     fp32 copy and runs logsumexp and gather: returns (log-probabilities fp32 [N], entropies fp32 [N] or None, row
     statistics fp32 [N, 4] for `token_logprobs_backward`).  `logits` [N, V] may be rows of a wider matrix; `targets` int64,
-    a negative one takes its row out (zeros), one outside the vocabulary gives NaN; `temperature` a number or fp32 [N]
-    (rows with a temperature <= 0 are scored at 1).  Rows of -inf only give -inf and entropy 0.  At most 2^22 rows."""
+    a negative one takes its row out (zeros), one outside the vocabulary gives NaN; `temperature` a number or fp32 [N] of
+    finite ones, no positive one below fp32's normal range (rows with a temperature <= 0 are scored at 1).  Rows of -inf only give -inf and entropy 0.  At most 2^22 rows."""
     temperatures, value = _check_logits(logits, targets, temperature)
     device, rows = _one_device(logits, targets, temperatures), logits.size(0)
     logprobs = logits.new_empty(rows, dtype=torch.float32)
@@ -955,7 +960,7 @@ class PolicyLossConfig:
     aggregate: str = "token"
 
     def __post_init__(self):
-        finite = lambda v: -float("inf") < float(v) < float("inf")
+        finite = lambda v: abs(float(v)) <= _FP32.max   # in the kernels' fp32
         reject(not 0.0 <= self.clip_low < 1.0, "clip_low must be in [0, 1)")
         reject(not (finite(self.clip_high) and self.clip_high >= 0.0), "clip_high must be finite and >= 0")
         reject(self.dual_clip is not None and not (finite(self.dual_clip) and self.dual_clip > 1.0), "dual_clip must be above 1")
@@ -1052,7 +1057,7 @@ def policy_gradient(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: t
     temperatures, value = _check_logits(logits, targets, temperature)
     tokens = logits.size(0)
     sequences = _check_tokens(tokens, old_logprobs, advantages, mask, ref_logprobs, cu_seqlens, per_sequence, config)
-    reject(not -float("inf") < float(grad_scale) < float("inf"), "grad_scale must be finite")
+    reject(not abs(float(grad_scale)) <= _FP32.max, "grad_scale must be finite")
     device = _one_device(logits, targets, temperatures, old_logprobs, advantages, mask, ref_logprobs, cu_seqlens)
     grad = _gradient_output(out, logits)
     fresh = old_logprobs.new_empty

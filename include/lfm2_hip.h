@@ -385,6 +385,7 @@ int lfm2_record_head(const int64_t* ids, const float* probs, int32_t* out_ids, f
  * m = max z and s = sum_v e^{(z_v - m) / T}:
  *   logprobs[n] = (z_target - m) / T - log s,   entropy[n] = log s - sum_v e^{(z_v - m) / T} (z_v - m) / T / s  (may be NULL),
  *   stats float[N, 4] = (m, log s, entropy or NaN, 0): what the gradient needs.
+ * A positive T is finite and not below the smallest normal float.
  * Rows are V consecutive elements, row_stride elements apart, at any element alignment.  targets int64[N]: a negative
  * one takes its row out (zeros, the row is not read); one >= V gives NaN.  A row of -inf only has no distribution:
  * log-probability -inf, entropy 0.  NaN or +inf in a row makes its results NaN.  Sums in fp32.  At most 2^22 rows here and
