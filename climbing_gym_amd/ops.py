@@ -1010,7 +1010,7 @@ def policy_loss_forward(logprobs: torch.Tensor, old_logprobs: torch.Tensor, adva
     device = _one_device(logprobs, old_logprobs, advantages, mask, ref_logprobs, entropy, cu_seqlens)
     fresh = old_logprobs.new_empty
     if tokens == 0:
-        return (torch.zeros((), device=device), torch.zeros(7, device=device), fresh(0), None if entropy is None else fresh(0))
+        return (old_logprobs.new_zeros(()), old_logprobs.new_zeros(7), fresh(0), None if entropy is None else fresh(0))
     loss, stats, grad = fresh(()), fresh(7), fresh(tokens)
     grad_entropy = None if entropy is None else fresh(tokens)
     workspace = fresh(_size("lfm2_policy_workspace", tokens, sequences, int(cu_seqlens is not None)))
@@ -1062,7 +1062,7 @@ def policy_gradient(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: t
     grad = _gradient_output(out, logits)
     fresh = old_logprobs.new_empty
     if tokens == 0:
-        return torch.zeros((), device=device), torch.zeros(7, device=device), fresh(0), grad
+        return old_logprobs.new_zeros(()), old_logprobs.new_zeros(7), fresh(0), grad
     loss, stats, logprobs = fresh(()), fresh(7), fresh(tokens)
     entropies = fresh(tokens) if config.entropy_coef != 0.0 else None
     workspace = fresh(_size("lfm2_policy_workspace", tokens, sequences, int(cu_seqlens is not None)))

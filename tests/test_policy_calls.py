@@ -33,3 +33,17 @@ def test_tokens_and_temperatures_that_inference_made_go_through_autograd():
     loss, _ = ops.policy_loss(logprobs, old, advantages)
     loss.backward()
     assert torch.equal(logprobs.grad, ops.policy_loss_forward(want[0], old, advantages)[2])
+
+
+@gpu
+def test_without_tokens_the_results_are_fp32_whatever_the_default_type_is():
+    row, logits = torch.zeros(0, device=DEV), torch.zeros(0, 9, device=DEV, dtype=torch.bfloat16)
+    targets = torch.zeros(0, device=DEV, dtype=torch.long)
+    torch.set_default_dtype(torch.float64)
+    try:
+        results = [*ops.policy_loss_forward(row, row, row, entropy=row), *ops.policy_gradient(logits, targets, row, row)[:3],
+                   ops.policy_loss(row.clone().requires_grad_(), row, row)[0]]
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(t.dtype == torch.float32 and (t == 0).all() for t in results)
+    assert [tuple(t.shape) for t in results] == [(), (7,), (0,), (0,), (), (7,), (0,), ()]
