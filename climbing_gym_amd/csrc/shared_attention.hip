@@ -1017,7 +1017,8 @@ int lfm2_shared_attention(void* out, const void* q, const void* k_cache, const v
   LFM2_REQUIRE(out && q && k_cache && v_cache && schedule && workspace, "shared_attention: null argument");
   LFM2_REQUIRE(!kv_fp8 || (k_scales && v_scales), "shared_attention: e4m3 history without scales");
   LFM2_REQUIRE(pools > 0, "shared_attention: empty cache");
-  LFM2_REQUIRE(scale > 0.f && scale <= 3.0e38f, "shared_attention: scale must be positive and finite");   // maxima are taken before it
+  // maxima are taken before the scale, and it is applied with log2(e)
+  LFM2_REQUIRE(scale > 0.f && scale * LFM2_LOG2E <= __FLT_MAX__, "shared_attention: scale must be positive and finite, with log2(e) too");
   LFM2_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)workspace | (uintptr_t)schedule) & 15) == 0,
                "shared_attention: tensors must be 16-byte aligned");
   LFM2_REQUIRE(!block_table || (page > 0 && max_blocks > 0 && max_blocks * (int64_t)page >= capacity), "shared_attention: bad page geometry");

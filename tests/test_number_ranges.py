@@ -47,3 +47,12 @@ def test_the_c_boundary(library):
         assert gradient(**kw) == -1 and text in message(), (kw, message())
     assert library.lfm2_policy_loss(p, p, p, None, p, p, p, p, None, None, None, p, 4, 1, 0, 0, 3, 0.2, 0.2, 0.0, math.inf, 0.0, None) == -1
     assert "coefficients" in message()
+
+
+def test_attention_scales_beyond_fp32(library):
+    """The kernels multiply by scale log2(e): 2.4e38 is a number of fp32, 2.4e38 x 1.44 is not."""
+    buffer = ctypes.create_string_buffer(4096 + 16)
+    p = (ctypes.addressof(buffer) + 15) // 16 * 16
+    for scale in (2.4e38, 3.4e38, math.inf, math.nan, 0.0, -1.0):
+        assert library.lfm2_shared_attention(p, p, p, p, None, None, p, None, 0, 16, p, 4, 8, 2, 64, 64, 4, 8192, 64, 64, scale, 0, 2, None) == -1, scale
+        assert "scale" in library.lfm2_last_error().decode()
