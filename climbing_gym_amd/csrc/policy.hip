@@ -791,7 +791,7 @@ int lfm2_token_logprobs(float* logprobs, float* entropy, float* stats, const voi
   DISPATCH_LOGITS(dtype,
     // 4096 rows of 4096 / 8192 values: 7.7 / 14.5 us with 128 threads, 11.7 / 16.2 with 512; of 65536: 85 and 83; 64 rows of
     // 16384: 5.2 and 4.2
-    const bool stream_once = N * row_stride * (int64_t)sizeof(T) >= kStreamBytes;
+    const bool stream_once = N * V * (int64_t)sizeof(T) >= kStreamBytes;   // what is read, however far apart the rows are
     if (V <= 8192) {
       if (stream_once) { if (entropy) LOGPROBS_(128, true, true); else LOGPROBS_(128, false, true); }
       else { if (entropy) LOGPROBS_(128, true, false); else LOGPROBS_(128, false, false); }
