@@ -267,6 +267,7 @@ struct LossArgs {
   const int64_t* targets;     // or null; a negative target takes its token out, like the mask
   const int32_t* cu;          // int32[S + 1], or null: one sequence of all N tokens
   const int32_t* counts;      // tokens that count, per sequence (per block of kCountBlock tokens without cu); null: all of them
+  const int32_t* totals;      // the batch's (tokens, sequences), or null: every workgroup sums the counts
   int64_t N, S, ncounts;
   int per_sequence, aggregate, kl;
   float clip_low, clip_high, dual_clip, kl_coef, entropy_coef;
@@ -341,24 +342,6 @@ __device__ __forceinline__ int sequence_count(const LossArgs& a, int64_t s) {
   const int64_t n = clamp_token(a.cu[s + 1], a.N) - clamp_token(a.cu[s], a.N);
   return n > 0 ? (int)n : 0;
 }
-// What every weight of the batch is divided by besides its sequence's count: all tokens that count, or the sequences that
-// have any.  `first` .. in steps of `step`: one thread's share of the sequences.
-struct Totals { int tokens, sequences; };
-__device__ __forceinline__ Totals partial_totals(const LossArgs& a, int first, int step) {
-  Totals t{0, 0};
-  for (int64_t s = first; s < a.ncounts; s += step) {
-    const int n = sequence_count(a, s);
-    t.tokens += n;
-    t.sequences += n > 0;
-  }
-  return t;
-}
-__device__ __forceinline__ float token_weight(const LossArgs& a, const Totals& total, int sequence_tokens) {
-  if (a.aggregate == LFM2_MEAN_SUM) return 1.f;
-  if (a.aggregate == LFM2_MEAN_SEQUENCES && a.cu) return (float)(1.0 / ((double)sequence_tokens * (double)total.sequences));
-  return (float)(1.0 / (double)total.tokens);
-}
-
 __device__ __forceinline__ int wave_sum_int(int v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
@@ -380,6 +363,31 @@ template <int WAVES> __device__ __forceinline__ int block_sum_int(int v, int* sc
   return t;
 }
 
+// What every weight of the batch is divided by besides its sequence's count: all tokens that count, or the sequences that
+// have any.  `first` .. in steps of `step`: one thread's share of the sequences.
+struct Totals { int tokens, sequences; };
+__device__ __forceinline__ Totals partial_totals(const LossArgs& a, int first, int step) {
+  Totals t{0, 0};
+  for (int64_t s = first; s < a.ncounts; s += step) {
+    const int n = sequence_count(a, s);
+    t.tokens += n;
+    t.sequences += n > 0;
+  }
+  return t;
+}
+template <int WAVES> __device__ __forceinline__ Totals batch_totals(const LossArgs& a, int* scratch) {
+  if (a.totals) return Totals{a.totals[0], a.totals[1]};
+  Totals t = partial_totals(a, threadIdx.x, 64 * WAVES);
+  t.tokens = block_sum_int<WAVES>(t.tokens, scratch);
+  t.sequences = block_sum_int<WAVES>(t.sequences, scratch);
+  return t;
+}
+__device__ __forceinline__ float token_weight(const LossArgs& a, const Totals& total, int sequence_tokens) {
+  if (a.aggregate == LFM2_MEAN_SUM) return 1.f;
+  if (a.aggregate == LFM2_MEAN_SEQUENCES && a.cu) return (float)(1.0 / ((double)sequence_tokens * (double)total.sequences));
+  return (float)(1.0 / (double)total.tokens);
+}
+
 // Tokens that count, per sequence (per block of kCountBlock tokens without sequences): one workgroup each.  This and the two
 // kernels after the next are chains of dependent loads, not of bytes: 16384 tokens of 64 sequences take 5, 11 and 4 us.
 __global__ void __launch_bounds__(256) policy_count_kernel(int32_t* counts, LossArgs a) {
@@ -391,6 +399,13 @@ __global__ void __launch_bounds__(256) policy_count_kernel(int32_t* counts, Loss
   for (int64_t t = begin + threadIdx.x; t < end; t += 256) n += (!a.mask || a.mask[t]) && (!a.targets || a.targets[t] >= 0);
   n = block_sum_int<4>(n, scratch);
   if (threadIdx.x == 0) counts[s] = n;
+}
+
+// Their totals, where there are too many counts for every workgroup to sum.
+__global__ void __launch_bounds__(1024) policy_totals_kernel(int32_t* totals, LossArgs a) {
+  __shared__ int scratch[16];
+  const Totals t = batch_totals<16>(a, scratch);
+  if (threadIdx.x == 0) { totals[0] = t.tokens; totals[1] = t.sequences; }
 }
 
 // The per-token part: gradients out, sums of the terms per workgroup.  Sums are kept in 64 bits and joined in a fixed
@@ -466,24 +481,33 @@ policy_tokens_kernel(LossArgs a, float* grad, float* grad_entropy, double* parti
 #pragma unroll
   for (int i = 0; i < PER; ++i) inputs[i].read(a, begin + threadIdx.x + 256 * i, end);
   const int64_t cu_first = a.cu ? a.cu[0] : 0, cu_last = a.cu ? a.cu[a.S] : a.N;
-  // one sweep over the sequences: the totals, and how many start at or before this range's first and last token
-  i32x4 n = {0, 0, 0, 0};
-  for (int64_t s = threadIdx.x; s < a.ncounts; s += 256) {
-    const int here = sequence_count(a, s);
-    n[0] += here;
-    n[1] += here > 0;
+  Totals total;
+  int64_t s_first = 0, s_last = a.S - 1;   // sequences that this range's tokens may belong to
+  if (a.totals) {
+    total = Totals{a.totals[0], a.totals[1]};
+  } else {
+    // one sweep over the sequences: the totals, and how many start at or before this range's first and last token
+    i32x4 n = {0, 0, 0, 0};
+    for (int64_t s = threadIdx.x; s < a.ncounts; s += 256) {
+      const int here = sequence_count(a, s);
+      n[0] += here;
+      n[1] += here > 0;
+      if (a.cu) {
+        n[2] += a.cu[s] <= begin;
+        n[3] += a.cu[s] < end;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = wave_sum_int(n[i]);
+    if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = n;
+    __syncthreads();
+    n = (counts[0] + counts[1]) + (counts[2] + counts[3]);
+    total = Totals{n[0], n[1]};
     if (a.cu) {
-      n[2] += a.cu[s] <= begin;
-      n[3] += a.cu[s] < end;
+      s_first = n[2] > 0 ? n[2] - 1 : 0;
+      s_last = n[3] > 0 ? n[3] - 1 : 0;
     }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) n[i] = wave_sum_int(n[i]);
-  if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = n;
-  __syncthreads();
-  n = (counts[0] + counts[1]) + (counts[2] + counts[3]);
-  const Totals total{n[0], n[1]};
-  const int64_t s_first = n[2] > 0 ? n[2] - 1 : 0, s_last = n[3] > 0 ? n[3] - 1 : 0;
   TermSums sums;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -502,7 +526,7 @@ policy_tokens_kernel(LossArgs a, float* grad, float* grad_entropy, double* parti
   sums.join<4>(scratch, out);
   __syncthreads();
   if (threadIdx.x < kLossTerms) partials[(int64_t)blockIdx.x * kLossTerms + threadIdx.x] = out[threadIdx.x];
-  if (blockIdx.x == 0 && threadIdx.x == 0) *tokens = total.tokens;
+  if (!a.totals && blockIdx.x == 0 && threadIdx.x == 0) *tokens = total.tokens;   // (the totals are there already)
 }
 __global__ void __launch_bounds__(256)
 policy_finish_kernel(LossArgs a, const double* partials, const int* tokens, int64_t blocks, float* loss, float* stats) {
@@ -636,9 +660,7 @@ __global__ void __launch_bounds__(THREADS) policy_gradient_kernel(GradientArgs a
   const float zt = (float)z[in_range ? target : 0];
   const float zl = has_tail ? (float)z[tail] : -kInf;
   // while the row is on its way: the token's weight
-  Totals total = partial_totals(a.loss, threadIdx.x, THREADS);
-  total.tokens = block_sum_int<THREADS / 64>(total.tokens, iscratch);
-  total.sequences = block_sum_int<THREADS / 64>(total.sequences, iscratch);
+  const Totals total = batch_totals<THREADS / 64>(a.loss, iscratch);
   const int64_t s = a.loss.cu ? sequence_of(a.loss.cu, 0, a.loss.S, row) : 0;
   const float w = token_weight(a.loss, total, a.loss.aggregate == LFM2_MEAN_SEQUENCES && a.loss.cu ? sequence_count(a.loss, s) : 0);
   const float old = a.loss.old[row], ref = a.loss.ref ? a.loss.ref[row] : 0.f, advantage = a.loss.advantages[a.loss.per_sequence ? s : row];
@@ -735,7 +757,7 @@ int fill_loss(const char* name, LossArgs* a, const float* logprobs, const float*
   LFM2_REQUIRE(clip_low >= 0.f && clip_low < 1.f && clip_high >= 0.f && clip_high <= 3.0e38f, "%s: clip range outside [0, 1) x [0, inf)", name);
   LFM2_REQUIRE(dual_clip == 0.f || (dual_clip > 1.f && finite(dual_clip)), "%s: dual_clip is 0 (off) or above 1", name);
   LFM2_REQUIRE(finite(kl_coef) && finite(entropy_coef), "%s: coefficients must be finite", name);
-  *a = LossArgs{logprobs, old, advantages, ref, entropy, mask, targets, cu, nullptr, N, cu ? S : 1, cu ? S : 1, per_sequence, aggregate, kl,
+  *a = LossArgs{logprobs, old, advantages, ref, entropy, mask, targets, cu, nullptr, nullptr, N, cu ? S : 1, cu ? S : 1, per_sequence, aggregate, kl,
                 clip_low, clip_high, dual_clip, kl_coef, entropy_coef, __builtin_log1p(-(double)clip_low),
                 __builtin_log1p((double)clip_high), dual_clip > 0.f ? __builtin_log((double)dual_clip) : 0.0};
   return LFM2_OK;
@@ -750,17 +772,28 @@ int64_t count_slots(int64_t N, int64_t S, bool cu) { return cu ? S : (N + kCount
 int64_t loss_blocks(int64_t N) { return (N + kLossTokens - 1) / kLossTokens; }
 // Workspace: the partial sums (64 bits, first for their alignment), the token count, the per-sequence counts.
 int64_t workspace_words(int64_t N, int64_t S, bool cu) { return 2 * loss_blocks(N) * kLossTerms + 2 + count_slots(N, S, cu); }
-struct LossWorkspace { double* partials; int *tokens, *counts; };
+struct LossWorkspace { double* partials; int *tokens, *counts; };   // tokens: two of them where they are the totals
 LossWorkspace split_workspace(float* ws, int64_t N) {
   double* partials = reinterpret_cast<double*>(ws);
   int* tokens = reinterpret_cast<int*>(partials + loss_blocks(N) * kLossTerms);
   return LossWorkspace{partials, tokens, tokens + 2};
 }
-void launch_counts(LossArgs* a, int* counts, hipStream_t s) {
-  if (!a->mask && !a->targets) return;   // every token counts: the bounds say how many
-  a->ncounts = count_slots(a->N, a->S, a->cu != nullptr);
-  hipLaunchKernelGGL(policy_count_kernel, dim3((unsigned)a->ncounts), dim3(256), 0, s, counts, *a);
-  a->counts = counts;
+// Up to so many counts every workgroup sums them itself; more are summed once, in a launch of their own (and a token's sequence
+// is looked for among all of them).  A workgroup of the loss has 1024 tokens, one of policy_gradient a row.  A loss of 2^18
+// masked tokens in 2048 / 4096 / 8192 sequences takes 18.7 / 22.9 / 31 us without that launch and 21.6 / 23.6 / 27 with it, of
+// 2^20 in 65536 146 and 78; policy_gradient of 8192 rows of 2048 values in 512 / 1024 / 4096 sequences 51 / 55 / 73 and 49 / 50 /
+// 57, of 32768 rows of 512 in 32768 505 and 153.
+constexpr int64_t kLossSweep = 4096, kRowSweep = 512;
+void launch_counts(LossArgs* a, int64_t sweep, const LossWorkspace& ws, hipStream_t s) {
+  if (a->mask || a->targets) {   // otherwise every token counts: the bounds say how many
+    a->ncounts = count_slots(a->N, a->S, a->cu != nullptr);
+    hipLaunchKernelGGL(policy_count_kernel, dim3((unsigned)a->ncounts), dim3(256), 0, s, ws.counts, *a);
+    a->counts = ws.counts;
+  }
+  if (a->ncounts > sweep) {
+    hipLaunchKernelGGL(policy_totals_kernel, dim3(1), dim3(1024), 0, s, ws.tokens, *a);
+    a->totals = ws.tokens;
+  }
 }
 bool single_workgroup(const LossArgs& a) { return a.N <= kSingleTokens && a.S <= kSingleSequences; }
 void launch_loss(const LossArgs& a, float* grad, float* grad_entropy, const LossWorkspace& ws, float* loss, float* stats, hipStream_t s) {
@@ -846,7 +879,7 @@ int lfm2_policy_loss(float* loss, float* stats, float* grad_logprobs, float* gra
   LFM2_REQUIRE(loss && stats && logprobs && workspace, "policy_loss: null argument");
   hipStream_t s = (hipStream_t)stream;
   const LossWorkspace ws = split_workspace(workspace, N);
-  if (!single_workgroup(a)) launch_counts(&a, ws.counts, s);
+  if (!single_workgroup(a)) launch_counts(&a, kLossSweep, ws, s);
   launch_loss(a, grad_logprobs, grad_entropy, ws, loss, stats, s);
   LFM2_LAUNCH_CHECK();
 }
@@ -872,7 +905,7 @@ int lfm2_policy_gradient(float* loss, float* stats, float* logprobs, float* entr
   g.grad_stride = grad_stride; g.stride = row_stride; g.V = V; g.temperature = temperature; g.grad_scale = grad_scale;
   hipStream_t s = (hipStream_t)stream;
   const LossWorkspace ws = split_workspace(workspace, N);
-  launch_counts(&g.loss, ws.counts, s);
+  launch_counts(&g.loss, kRowSweep, ws, s);
 #define GRADIENT_(THREADS, VECS)                                                                                                  \
   do {                                                                                                                            \
     if (entropy) hipLaunchKernelGGL((policy_gradient_kernel<T, THREADS, VECS, true>), dim3((unsigned)N), dim3(THREADS), 0, s, g);  \

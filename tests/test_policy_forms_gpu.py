@@ -54,20 +54,20 @@ def test_rows_of_a_very_wide_matrix(ops):
 #   H = log s - sum(e d) / s: S + 4 M2 + 160 M1 + 2 l;
 #   the slope of the loss by 16 of w (|A| r + kl (1 + e^x)) (exponentials 2 each after arguments right to a rounding of at
 #   most 2, products and constants 1 each), the factors 1 / T, w and the sums 8.
-def _check_long_rows(ops, dtype, v, entropy_coef, rows=12, seed=1):
+def _check_long_rows(ops, dtype, v, entropy_coef, rows=12, seed=1, bounds=None, aggregate="sequence"):
     from test_policy_gpu import U, _definition, _plain
     g = torch.Generator(device=DEV).manual_seed(seed + v)
     logits = (3 * torch.randn(rows, v, device=DEV, generator=g)).to(dtype)
     targets = torch.randint(0, v, (rows,), device=DEV, generator=g)
     targets[0], targets[1], targets[5] = v - 1, 0, -1
-    bounds = [0, 4, 4, rows - 1]                                       # one row behind the last sequence
+    bounds = bounds or [0, 4, 4, rows - 1]                             # one row behind the last sequence
     mask = torch.ones(rows, dtype=torch.bool, device=DEV)
     mask[2] = False
     t = 0.9
     lp, h, d, logs, p, _ = _plain(logits, targets, t)
     normal = lambda: torch.randn(rows, device=DEV, generator=g)
     old, ref, adv = (lp + 0.2 * normal()).float(), (lp + 0.2 * normal()).float(), normal()
-    cfg = ops.PolicyLossConfig(clip_low=0.2, clip_high=0.3, kl_coef=0.1, entropy_coef=entropy_coef, aggregate="sequence")
+    cfg = ops.PolicyLossConfig(clip_low=0.2, clip_high=0.3, kl_coef=0.1, entropy_coef=entropy_coef, aggregate=aggregate)
     kw = dict(mask=mask, ref_logprobs=ref, cu_seqlens=torch.tensor(bounds, dtype=torch.int32, device=DEV), config=cfg, temperature=t)
     loss, stats, logprobs, grad = ops.policy_gradient(logits, targets, old, adv, **kw)
     live = mask & (targets >= 0)
@@ -85,10 +85,13 @@ def _check_long_rows(ops, dtype, v, entropy_coef, rows=12, seed=1):
     x, hh = cpu(logprobs).requires_grad_(), cpu(h).requires_grad_()
     want, want_stats = _definition(x, cpu(old), cpu(adv), live.cpu(), cpu(ref), hh if entropy_coef else None, bounds, cfg)
     slope, hslope = torch.autograd.grad(want, (x, hh), allow_unused=True)
-    w = torch.zeros(rows, dtype=torch.float64, device=DEV)
-    for a, b in zip(bounds[:-1], bounds[1:]):
-        if live[a:b].any():
-            w[a:b] = live[a:b].double() / (live[a:b].sum() * 2)
+    host = live.cpu()
+    counts = [int(host[a:b].sum()) for a, b in zip(bounds[:-1], bounds[1:])]
+    total, used = sum(counts), sum(c > 0 for c in counts)
+    w = torch.zeros(rows, dtype=torch.float64)
+    for a, b, c in zip(bounds[:-1], bounds[1:], counts):
+        w[a:b] = {"sequence": 1.0 / (max(c, 1) * used), "token": 1.0 / total, "sum": 1.0}[aggregate]
+    w = torch.where(live, w.to(DEV), 0.0)
     ratio, other = (logprobs.double() - old.double()).exp(), (ref.double() - logprobs.double()).exp()
     size = w * (adv.double().abs() * ratio + 0.1 * (1 + other))
     eh = s + U * (4 * m2 + 160 * m1 + 2 * l)
@@ -133,3 +136,64 @@ def test_policy_gradient_of_long_rows_in_place_and_inside_a_wider_matrix(ops, dt
     assert again[3] is inside
     for x, y in zip(again[:3], (loss, stats, logprobs)):
         assert torch.equal(x, y)
+
+
+# --------------------------------------------------------------------------------------------- many sequences
+def _random_bounds(n, sequences, end):
+    g = torch.Generator().manual_seed(sequences)
+    return [0, *torch.randint(0, end + 1, (sequences - 1,), generator=g).sort().values.tolist(), end]
+
+
+@pytest.mark.parametrize("n, sequences", ((3000, 512), (3000, 513), (3000, 4097), (9000, 20000)))
+@pytest.mark.parametrize("aggregate", ("token", "sequence", "sum"))
+def test_policy_gradient_over_many_sequences(ops, n, sequences, aggregate):
+    _check_long_rows(ops, torch.float32, 37, 0.02, rows=n, bounds=_random_bounds(n, sequences, n - 1), aggregate=aggregate)
+
+
+@pytest.mark.parametrize("n, sequences", ((3000, 4097), (20000, 4096), (20000, 4097), (70001, 6000), (5000, 70000)))
+@pytest.mark.parametrize("aggregate", ("token", "sequence", "sum"))
+@pytest.mark.parametrize("masked, per_sequence", ((False, False), (True, True)))
+def test_policy_loss_over_many_sequences(ops, n, sequences, aggregate, masked, per_sequence):
+    from test_policy_gpu import U, _definition, _tokens
+    lp, old, a, mask, _, _ = _tokens(n, sequences)
+    bounds = _random_bounds(n, sequences, n - 7)
+    which = torch.zeros(n, dtype=torch.long)
+    for i, (s, e) in enumerate(zip(bounds[:-1], bounds[1:])):
+        which[s:e] = i
+    adv = torch.randn(sequences, generator=torch.Generator().manual_seed(n)) if per_sequence else a
+    token_adv = adv[which] if per_sequence else adv
+    cfg = ops.PolicyLossConfig(aggregate=aggregate)
+    x = lp.double().requires_grad_()
+    want, stats = _definition(x, old.double(), token_adv.double(), mask if masked else torch.ones(n, dtype=torch.bool), None, None, bounds, cfg)
+    slope, = torch.autograd.grad(want, x)
+    got = ops.policy_loss_forward(lp.to(DEV), old.to(DEV), adv.to(DEV), mask=mask.to(DEV) if masked else None, per_sequence=per_sequence, config=cfg,
+                                  cu_seqlens=torch.tensor(bounds, dtype=torch.int32, device=DEV))
+    # a token's slope: exponential |d| + 2 <= 10, products 2: 12 u; a loss of as many terms, none larger than r |A| w or 1.2 |A| w
+    assert ((got[2].double().cpu() - slope).abs() <= 12 * U * slope.abs()).all() and (got[2][bounds[-1]:] == 0).all()
+    counted = (mask if masked else torch.ones(n, dtype=torch.bool)).double()
+    counted[bounds[-1]:] = 0
+    w = {"sum": counted, "token": counted / counted.sum()}.get(aggregate)
+    if w is None:
+        per = torch.zeros(sequences, dtype=torch.float64).index_add_(0, which[:bounds[-1]], counted[:bounds[-1]])
+        w = counted / (per.clamp_min(1)[which] * (per > 0).sum())
+    size = (w * (lp.double() - old.double()).exp().clamp_min(1.2) * token_adv.double().abs()).sum()
+    assert abs(got[0].double().cpu() - want.detach()) <= 12 * U * size + U * want.abs()
+    assert got[1][6].item() == counted.sum()
+
+
+def test_policy_loss_of_one_sequence_of_many_tokens(ops):
+    """More blocks of counted tokens than a workgroup sweeps, without sequences: 2^24 + 2^13 tokens."""
+    from test_policy_gpu import U
+    n = (1 << 24) + (1 << 13) + 5
+    g = torch.Generator(device=DEV).manual_seed(3)
+    normal = lambda: torch.randn(n, device=DEV, generator=g)
+    old, adv, mask = -normal().abs(), normal(), normal() > -0.5
+    lp = old + 0.1 * normal()
+    loss, stats, grad, _ = ops.policy_loss_forward(lp, old, adv, mask=mask, config=ops.PolicyLossConfig(clip_high=0.25, clip_low=0.25))
+    ratio, a, w = (lp.double() - old.double()).exp(), adv.double(), mask.double() / mask.sum()
+    gain = torch.minimum(ratio * a, ratio.clamp(0.75, 1.25) * a)
+    want = -(w * gain).sum()
+    assert stats[6].item() == mask.sum()
+    assert abs(loss.double() - want) <= 12 * U * (w * gain.abs()).sum() + U * want.abs()
+    slope = torch.where(ratio.clamp(0.75, 1.25) * a < ratio * a, 0.0, -w * ratio * a)
+    assert ((grad.double() - slope).abs() <= 12 * U * slope.abs()).all()
