@@ -12,7 +12,8 @@ Reference module -> module of this package:
 from .config import LFM2Config, LFM25SamplingConfig
 
 __all__ = ["LFM2Config", "LFM25SamplingConfig", "LFM25Engine", "LFM25PackedWeights", "LFM25HybridCache",
-           "LFM25PrefixBatch", "LFM25DecodeBatch", "LFM25StepOutput", "LFM25GenerationOutput", "LFM25HIPDecoder",
+           "LFM25PrefixBatch", "LFM25DecodeBatch", "LFM25StepOutput", "LFM25GenerationOutput", "LFM25PolicyObjective",
+           "LFM25HIPDecoder",
            "LFM25CUDADecoder", "LFM25GenerationSession", "LFM25ContinuationHandle", "LFM25SessionResult",
            "flatten_token_batches", "LFM25AsyncInferenceEngine", "SamplingConfig", "InferenceEngineConfig",
            "GenerationOutput", "GenerationResult", "RolloutRunner", "RolloutRunnerConfig", "RolloutConfig",
@@ -20,7 +21,7 @@ __all__ = ["LFM2Config", "LFM25SamplingConfig", "LFM25Engine", "LFM25PackedWeigh
 
 _LAZY = {
     "LFM25Engine": "engine", "LFM25PrefixBatch": "engine", "LFM25DecodeBatch": "engine", "LFM25StepOutput": "engine",
-    "LFM25GenerationOutput": "engine", "flatten_token_batches": "engine", "LFM25PackedWeights": "weights",
+    "LFM25GenerationOutput": "engine", "LFM25PolicyObjective": "engine", "flatten_token_batches": "engine", "LFM25PackedWeights": "weights",
     "LFM25HybridCache": "cache", "LFM25HIPDecoder": "decoder", "LFM25CUDADecoder": "decoder",
     "LFM25GenerationSession": "session", "LFM25ContinuationHandle": "session", "LFM25SessionResult": "session",
     "LFM25AsyncInferenceEngine": "async_engine", "SamplingConfig": "inference_config",

@@ -71,3 +71,10 @@ def test_refused_before_any_prefill(args, kw, text):
 def test_what_is_right_gets_as_far_as_the_prefill():
     with pytest.raises(Reached):
         Engine().policy_objective(PROMPTS, COMPLETIONS, OLD, torch.ones(3))
+
+
+def test_the_package_offers_what_a_call_returns():
+    import climbing_gym_amd
+    from climbing_gym_amd.engine import LFM25PolicyObjective
+    assert climbing_gym_amd.LFM25PolicyObjective is LFM25PolicyObjective and "LFM25PolicyObjective" in climbing_gym_amd.__all__
+    assert all(hasattr(climbing_gym_amd, name) for name in climbing_gym_amd.__all__)
