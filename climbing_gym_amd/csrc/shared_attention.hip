@@ -398,7 +398,8 @@ __device__ __forceinline__ bool list_fits(const SharedArgs& a, int D) {
 // reference point cancels in the end.
 // The second product takes 16-bit operands.  A 16-bit history's P goes in as two of them, the rounded value and the rounded
 // rest (2^-16 relative in bf16: one rounding alone would be as large as the output's own).  An e4m3 history's goes in as one
-// fp16 value (2^-12), with the scale of its V row: the weight is w = 2^{s + log2 vs - m}, m a running maximum of s + log2 vs,
+// fp16 value (2^-11, and 2^-25 of the largest weight below fp16's normal range: less than a bf16 output's own rounding, as much
+// as an fp16 one's), with the scale of its V row: the weight is w = 2^{s + log2 vs - m}, m a running maximum of s + log2 vs,
 // so it stays in fp16's range whatever the scales are, and the softmax sum takes w / vs.
 template <typename T, bool FP8, int D> struct Shape {
   typedef std::conditional_t<FP8, _Float16, T> P;   // type of P and V: fp16 holds e4m3 exactly, and three more bits of P than bf16
@@ -802,8 +803,8 @@ __device__ __forceinline__ void block_item(const SharedArgs& a, const i32x4 r0, 
 // A shared item: up to 64 queries of a group against tokens [t0, t1) of one KV head, 128 tokens at a time.  All four waves
 // stage the tile (the next one is on its way to registers meanwhile); then each takes NB query blocks against its share of the
 // tile's tokens: the waves of one set of blocks share them evenly, and their results meet at the end.  An e4m3 history takes
-// two blocks a wave (32 x 16 rows, 5500 shared tokens: 73 us against 79 with one), since each is read with three scales per
-// token; a 16-bit one takes one block and twice the tokens at a time (85 us against 90: the weights' second part and the
+// two blocks a wave (32 x 16 rows, 5500 shared tokens: 8 % less time than one block), since each is read with three scales per
+// token; a 16-bit one takes one block and twice the tokens at a time (6 % less time than two: the weights' second part and the
 // wider rows in flight need the registers).
 template <typename T, bool FP8, bool PAGED, int D>
 __device__ __forceinline__ void shared_item(const SharedArgs& a, const i32x4 r0, const i32x4 r1, int h, bf16x8* lds, float* lds_scale) {
@@ -865,10 +866,13 @@ __device__ __forceinline__ void shared_item(const SharedArgs& a, const i32x4 r0,
   }
 }
 
-// Own parts alone (256 rows of 2000 tokens, 8 KV heads of 64 dims): 177 us in bf16, 6.1 TB/s; 113 in e4m3, 5.1 TB/s, where
-// the three waves a SIMD has registers for do not ask for enough bytes.  Shared parts alone (32 x 16 rows, 5500 tokens, 23
-// GFLOP, 90 M exponentials): 77 and 70 us with the join, bound by LDS reads and vector
-// instructions per score (e4m3: loads alone 45, arithmetic alone 56, with staging 65).
+// Own parts alone (256 rows of 2000 tokens, 8 KV heads of 64 dims), this launch and the join's 5 us: 184 us in bf16 (5.9 TB/s in
+// this one), 119 in e4m3 (4.9).  Both have three waves a SIMD with 4 KiB each of K and of V; a tile of e4m3 is 64 tokens, and
+// the next one is asked for when the second half of it has been staged, so that nothing is on its way during the first, while a
+// 16-bit tile of 32 tokens is replaced as soon as it has been staged.  (`attend` on the same rows: 162 and 94.)  Shared parts
+// alone (32 x 16 rows, 5500 tokens, 23 GFLOP, 90 M exponentials), with the join: 87 us in bf16, 65 in e4m3, bound by LDS reads
+// and vector instructions per score (an earlier e4m3 build of 70 us took 45 for loads alone, 56 for arithmetic alone and 65 for
+// arithmetic and staging).
 template <typename T, bool FP8, bool PAGED, int D>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 64 ? 3 : 2))) shared_attention_kernel(SharedArgs a) {
   typedef Shape<T, FP8, D> S;
@@ -892,8 +896,9 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 6
   // The first 2 * shared_blocks workgroups take shared and other items in turn, the rest other items: what runs at the same
   // time on a CU is some of each (shared parts are bound by arithmetic, the others by memory).  A turn is one workgroup for
   // every CU: consecutive workgroups go to the XCDs, their shader engines and CUs in turn, so that a shorter period would
-  // give all shared items to some of them (32 x 16 rows, 5500 shared tokens: turns of 8 workgroups 108 us in e4m3 and 115 in bf16, of 256 74 and 85).  The grid fills the
-  // chip about once and strides over the items: a workgroup without work costs its slot a microsecond or two.
+  // give all shared items to some of them (32 x 16 rows, 5500 shared tokens: turns of 256 workgroups take 69 % of the time that
+  // turns of 8 take in e4m3, 74 % in bf16).  The grid fills the chip about once and strides over the items: a workgroup without
+  // work costs its slot a microsecond or two.
   int block = blockIdx.x;
   if (block < 2 * a.shared_blocks && block % (2 * kTurn) < kTurn) {
     for (int idx = block / (2 * kTurn) * kTurn + block % kTurn; idx < shared_records * a.KH; idx += a.shared_blocks) {

@@ -230,8 +230,11 @@ class LFM25Engine:
                            shared_prefix: bool = False) -> None:
         """Same switch as the reference (lfm25_engine.py:980-997); graphs are HIP graphs.  `fp8_operators` extends
         W8A8 to the QKV/out and conv in/out projections; `bf16_weight_packing` is accepted and ignored.  With
-        `shared_prefix`, `generate` with repeats keeps one copy of a prompt's keys and values and reads it once per step for
-        all its completions."""
+        `shared_prefix`, `generate` with repeats writes one copy of a prompt's keys and values and reads it once per step for
+        all its completions.  That pays where completions are not much longer than their prompt: with 16 completions of a
+        prompt of 256 tokens up to about 500 tokens each (250 with an e4m3 history), of 1000 tokens and more at any length
+        up to 8000; beyond that it costs up to a fifth of the attention's time.  Every row's slot is allocated as without it.
+        Sessions, and what runs on them (the async engine, rollouts), prefill each prompt on its own and do not share."""
         from .decoder import LFM25HIPDecoder
         reject(self._decoder_busy, "Close the native generation session before reconfiguring CUDA graphs", RuntimeError)
         if self._cuda_decoder is not None:
@@ -590,7 +593,8 @@ class LFM25Engine:
     def fork(self, prefix: LFM25PrefixBatch, repeats: int, *, max_cache_len: int | None = None,
              share_prefix: bool = False) -> LFM25DecodeBatch:
         """Every prompt `repeats` times (lfm25_engine.py:761).  With `share_prefix` only the first repeat of a prompt gets
-        its keys and values; the others read them there (`ops.attend_shared`), once for all of them per step."""
+        its keys and values; the others read them there (`ops.attend_shared`), once for all of them per step.  Their slots
+        are allocated all the same: what is saved is copies and reads, not memory."""
         reject(repeats <= 0, "repeats must be > 0")
         reject(share_prefix and self.dtype not in (torch.bfloat16, torch.float16), "shared prefixes need a bf16 or fp16 model")
         prompts = prefix.batch_size
