@@ -867,7 +867,8 @@ def token_logprobs_forward(logits: torch.Tensor, targets: torch.Tensor, *, tempe
     fp32 copy and runs logsumexp and gather: returns (log-probabilities fp32 [N], entropies fp32 [N] or None, row
     statistics fp32 [N, 4] for `token_logprobs_backward`).  `logits` [N, V] may be rows of a wider matrix; `targets` int64,
     a negative one takes its row out (zeros), one outside the vocabulary gives NaN; `temperature` a number or fp32 [N] of
-    finite ones, no positive one below fp32's normal range (rows with a temperature <= 0 are scored at 1).  Rows of -inf only give -inf and entropy 0.  At most 2^22 rows."""
+    finite ones, no positive one below fp32's normal range (rows with a temperature <= 0 are scored at 1).  Rows of -inf only
+    give -inf and entropy 0.  At most 2^22 rows."""
     temperatures, value = _check_logits(logits, targets, temperature)
     device, rows = _one_device(logits, targets, temperatures), logits.size(0)
     logprobs = logits.new_empty(rows, dtype=torch.float32)
